@@ -536,6 +536,71 @@ int nvk_sample(const void* logits, int64_t row_stride, int32_t batch, int32_t vo
                int64_t noise_row_stride, uint64_t seed, uint64_t offset, int64_t* tokens,
                void* workspace, size_t workspace_bytes, void* stream);
 
+/*
+ * The 4-bit key/value cache.  No counterpart in the reference, whose caches are the model's 16-bit
+ * type (nanovllm/engine/model_runner.py:115-121).  Per layer, for keys and for values each, with
+ * D = head_dim and P = block_size (contiguous, 16-byte aligned):
+ *   data   uint8 [num_blocks][num_kv_heads][P][D / 2]   two codes a byte, the lower nibble first
+ *   scale  f16   [num_blocks][num_kv_heads][D / 32][P]
+ * A code is a sign bit and three bits that stand for 0, 0.5, 1, 1.5, 2, 3, 4, 6 (e2m1).  The 32
+ * dimensions 32 s .. 32 s + 31 share scale = f16(min(max|x| / 6, 65504)); every value takes the
+ * code nearest to x / scale (ties to the even code, beyond 6: 6) and stands for code * scale.  A
+ * group whose scale rounds to 0 holds zeros; one with an infinity or NaN has the scale NaN and stands
+ * for NaN.  A row of values holds its dimensions in order; a row of keys holds them in units of 8
+ * (4 bytes): unit 32 s + 8 g .. + 7 at place (D / 32) g + s (g < 4).
+ * Slot s = page * P + offset, as in the 16-bit caches.  head_dim: 128 or 64.  block_size: a
+ * multiple of 16.  dtype (of the 16-bit rows): NVK_DTYPE_BF16 or NVK_DTYPE_F16.
+ *
+ * nvk_fp4_store: nvk_kv_store into such caches: row slot_mapping[t] of every head = what the
+ *   format makes of key[t], value[t] (row t at t * row_stride, heads contiguous; rows 16-byte
+ *   aligned, strides multiples of 8 elements).  Slots outside [0, num_blocks * block_size)
+ *   are skipped; of several tokens with one slot one wins.
+ * nvk_fp4_load: key[t], value[t] = the rows of slot_mapping[t], every value rounded once to dtype;
+ *   zeros where the slot lies outside the cache.
+ * Each is one kernel.
+ */
+int nvk_fp4_store(const void* key, int64_t key_row_stride, const void* value,
+                  int64_t value_row_stride, void* k_data, void* k_scale, void* v_data,
+                  void* v_scale, const int32_t* slot_mapping, int64_t n_tokens,
+                  int32_t num_kv_heads, int32_t head_dim, int32_t block_size, int32_t num_blocks,
+                  int32_t dtype, void* stream);
+int nvk_fp4_load(const void* k_data, const void* k_scale, const void* v_data, const void* v_scale,
+                 const int32_t* slot_mapping, int64_t n_tokens, int32_t num_kv_heads,
+                 int32_t head_dim, int32_t block_size, int32_t num_blocks, void* key,
+                 int64_t key_row_stride, void* value, int64_t value_row_stride, int32_t dtype,
+                 void* stream);
+
+/*
+ * Causal attention of each sequence's last tokens over the 4-bit cache: what nvk_paged_decode,
+ * nvk_paged_verify and the paged nvk_varlen_prefill are to the 16-bit ones.
+ *
+ * cu_seqlens_q == NULL: max_seqlen_q queries per sequence (total_q = batch * max_seqlen_q),
+ *   seqlens_k [batch] its keys (context lengths, the queries' own tokens among them).
+ * Otherwise both are prefix sums [batch + 1], as in nvk_varlen_prefill; queries past
+ *   max_seqlen_q, and sequences that do not lie within q's total_q rows, are left unwritten.
+ * Query i of Lq sees key j iff j <= i + Lk - Lq; one that sees none is written as zeros.
+ * q, out, block_tables, scale: as in nvk_paged_decode.  A page id outside [0, num_blocks) is never
+ *   followed; the output of a sequence that names one is unspecified.
+ * The scores are f32 sums of exact products; a probability times its value's scale is rounded to
+ *   f16 before the product with the codes, whose sums are f32.
+ * G = num_q_heads / num_kv_heads: at most 16.  batch <= 2048.
+ * workspace: device scratch of nvk_fp4_attention_workspace_size() bytes, 256-byte aligned, not
+ *   initialised; two calls in flight at once need two.  The size is 0 for sizes that are not
+ *   supported (the call returns NVK_EUNSUPPORTED).  Two kernels.
+ */
+size_t nvk_fp4_attention_workspace_size(int32_t batch, int32_t max_seqlen_q, int32_t num_q_heads,
+                                        int32_t num_kv_heads, int32_t head_dim,
+                                        int32_t block_size, int32_t max_blocks);
+int nvk_fp4_attention(const void* q, int64_t q_stride_tok, int64_t q_stride_head, int64_t total_q,
+                      const void* k_data, const void* k_scale, const void* v_data,
+                      const void* v_scale, const int32_t* cu_seqlens_q, const int32_t* seqlens_k,
+                      int32_t batch, int32_t max_seqlen_q, const int32_t* block_tables,
+                      int64_t bt_stride, int32_t max_blocks, int32_t block_size,
+                      int32_t num_blocks, int32_t num_q_heads, int32_t num_kv_heads,
+                      int32_t head_dim, float scale, void* out, int64_t out_stride_tok,
+                      int64_t out_stride_head, void* workspace, size_t workspace_bytes,
+                      int32_t dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

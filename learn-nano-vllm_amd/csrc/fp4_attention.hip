@@ -1,0 +1,673 @@
+// Attention over the 4-bit cache (layout: fp4.h): the queries are the last ones of their sequence's
+// keys, one per sequence (a decode step) or several (verification, a chunk of a prompt).
+//
+//   s_j = scale * sum_g ks[j, g] * (q_g . kc[j, g])      over the 32-dimension groups g
+//   o   = sum_j p_j vs[j, g] vc[j, g] / sum_j p_j        p = softmax over the visible keys
+//
+// The codes kc, vc are exact in bf16 and f16, so they are what the matrix instructions multiply, and
+// the scales are applied to the products: to the f32 sums of a key's groups (S), and to
+// the probabilities (P.V), which become one operand per group.
+//   * A wave owns 16 rows (query token x query head of a kv head) and streams their keys in chunks
+//     of 64; the chunks of all (sequence, kv head, 16-row tile) groups are cut into equal
+//     contiguous ranges, one per wave.  Groups cut between waves leave (O, m, l) records that a
+//     second kernel merges.
+//   * S^T = K Q^T on v_mfma_f32_16x16x32: operand row m = 4 a + i of key block b is key
+//     16 a + 4 b + i of the chunk, so lane (g, r) ends up with the scores of keys 16 g .. +15 of
+//     row r in order: the order in which ds_read_b64_tr_b4 hands it the values of a dimension.
+//   * O^T = V^T P^T likewise, V^T read transposed from LDS by ds_read_b64_tr_b4.
+//   * The probabilities times vs are rounded to f16 for both types of model: 2^-11 relative (bf16: 2^-8),
+//     and p <= 1, so that nothing overflows.  Below 2^-14 the step is 2^-24, no coarser than that of
+//     the scales themselves.
+//   * A chunk's keys go to registers, its values and scales to LDS (DMA), all one chunk ahead.
+#include <type_traits>
+
+#include "fp4.h"
+
+namespace {
+
+constexpr int kR = 16;                   // rows of a tile
+constexpr int kCK = 64;                  // keys of a chunk
+constexpr int kWavesPerWG = 4;
+constexpr int kMaxWGs = 512;             // two workgroups per CU
+constexpr int kMaxBatch = 2048;
+
+typedef __attribute__((address_space(4))) const int32_t const_i32;
+typedef __attribute__((address_space(3))) void* lds_ptr;
+typedef int i32x2 __attribute__((ext_vector_type(2)));
+
+struct AttnArgs {
+  const uint16_t* q;
+  int64_t q_stride_tok, q_stride_head, total_q;
+  const uint8_t *k_data, *v_data;
+  const uint16_t *k_scale, *v_scale;
+  const int32_t* cu_q;   // null: n_query queries per sequence, keys[s] its context length
+  const int32_t* keys;   // cu_seqlens_k, or context lengths
+  const int32_t* block_tables;
+  int64_t bt_stride;
+  int batch, n_query, max_tiles, cap, block_size, num_blocks;
+  int num_kv_heads, G;
+  float scale_log2;
+  uint16_t* out;
+  int64_t out_stride_tok, out_stride_head;
+  int32_t* desc;  // [batch][Hkv][max_tiles] x 2: first and last wave of the group, -1 if empty
+  float* rec;     // [n_waves][2][rec_rows][HD + 4]: O, m, l
+  int rec_rows, n_waves;
+};
+
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// Queries, their first row and the keys of sequence s (cu_q beyond what q holds is not followed).
+struct Seq {
+  int row0, queries, raw_keys, keys;
+};
+__device__ __forceinline__ Seq seq_of(const AttnArgs& a, int s) {
+  Seq x;
+  if (a.cu_q) {
+    const const_i32* cq = (const_i32*)a.cu_q;
+    const const_i32* ck = (const_i32*)a.keys;
+    x.row0 = cq[s];
+    x.queries = cq[s + 1] - x.row0;
+    x.raw_keys = ck[s + 1] - ck[s];
+    if (x.queries > a.n_query) x.queries = a.n_query;
+    if (x.row0 < 0 || x.queries < 0 || (int64_t)x.row0 + x.queries > a.total_q) x.queries = 0;
+  } else {
+    x.row0 = s * a.n_query;
+    x.queries = a.n_query;
+    x.raw_keys = ((const_i32*)a.keys)[s];
+  }
+  x.keys = x.raw_keys < 0 ? 0 : x.raw_keys;
+  if (x.keys > a.cap) x.keys = a.cap;
+  return x;
+}
+__device__ __forceinline__ int tiles_of(const AttnArgs& a, const Seq& x) {
+  return (x.queries * a.G + kR - 1) / kR;
+}
+__device__ __forceinline__ int chunks_of(const Seq& x) { return (x.keys + kCK - 1) / kCK; }
+__device__ __forceinline__ int seq_units(const AttnArgs& a, int s) {
+  const Seq x = seq_of(a, s);
+  return tiles_of(a, x) * chunks_of(x);
+}
+
+// Exclusive prefix of the sequences' (tile, chunk) pairs into s_cs[0..B]; returns the total.
+__device__ int unit_prefix(const AttnArgs& a, int* s_cs, int* s_wsum) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int B = a.batch;
+  const int per = (B + 255) / 256;
+  const int b0 = tid * per;
+  int local = 0;
+  for (int i = 0; i < per; ++i)
+    if (b0 + i < B) local += seq_units(a, b0 + i);
+  const int x = nvk_wave_scan_add(local);
+  if (lane == 63) s_wsum[wave] = x;
+  __syncthreads();
+  int run = x - local;
+  for (int w = 0; w < wave; ++w) run += s_wsum[w];
+  for (int i = 0; i < per; ++i) {
+    if (b0 + i < B) {
+      s_cs[b0 + i] = run;
+      run += seq_units(a, b0 + i);
+    }
+  }
+  const int total = s_wsum[0] + s_wsum[1] + s_wsum[2] + s_wsum[3];
+  if (tid == 0) s_cs[B] = total;
+  __syncthreads();
+  return total;
+}
+
+__device__ __forceinline__ int64_t active_waves(int64_t T, int64_t P) {
+  return T < P ? (T < 1 ? 1 : T) : P;
+}
+__device__ __forceinline__ int64_t range_begin(int64_t w, int64_t T, int64_t P) { return w * T / P; }
+__device__ __forceinline__ int64_t chunk_owner(int64_t c, int64_t T, int64_t P) {
+  return ((c + 1) * P - 1) / T;
+}
+
+// 16 bytes per lane from its own address straight into LDS: lane l writes [dst + 16 l, +16).
+__device__ __forceinline__ void lds_load(const void* src, uint32_t dst) {
+  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off nt"
+               :: "v"(src), "s"(dst) : "memory", "m0");
+}
+// Every load has landed and every LDS read of the buffers about to be refilled is done.
+__device__ __forceinline__ void wait_all() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+}
+
+__device__ __forceinline__ float sum_xor16(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float max_xor16(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+template <int HD>
+struct KeyVec;
+template <>
+struct KeyVec<128> {
+  typedef nvk_u32x4 type;
+};
+template <>
+struct KeyVec<64> {
+  typedef nvk_u32x2 type;
+};
+
+// ONEPAGE: pages of a multiple of 64 keys, so that a chunk lies in one; else of a multiple of 16.
+template <int HD, bool F16, bool ONEPAGE>
+__global__ __launch_bounds__(64 * kWavesPerWG, 2) void fp4_attention_kernel(AttnArgs a) {
+  using E = NvkElt<F16>;
+  typedef typename E::vec8 vec8;
+  typedef typename KeyVec<HD>::type kvec;
+  constexpr int NG = HD / kFp4Group;       // scale groups = MFMA k-steps of S
+  constexpr int RB = HD / 2;               // bytes of a row of codes
+  constexpr int kVBytes = kCK * RB;        // a chunk's values in LDS
+  constexpr int kBuf = kVBytes + 1024;     // and its scales (D = 64 uses half of the 1024)
+  constexpr int kBlk = ONEPAGE ? 1 : 4;    // pages looked up per chunk
+  constexpr int kRec = HD + 4;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[kWavesPerWG * 2 * kBuf];
+  __shared__ int s_cs[kMaxBatch + 1];
+  __shared__ int s_wsum[kWavesPerWG];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int r = lane & 15, g = lane >> 4;
+  const int Hkv = a.num_kv_heads;
+
+  const int S = unit_prefix(a, s_cs, s_wsum);
+  if (blockIdx.x == 0) {  // groups that no wave visits
+    const int per = Hkv * a.max_tiles;
+    for (int e = tid; e < a.batch * per; e += 256) {
+      const int b = e / per;
+      if (s_cs[b + 1] == s_cs[b])
+        *reinterpret_cast<int2*>(a.desc + 2 * (int64_t)e) = make_int2(-1, -1);
+    }
+  }
+  const int64_t T = (int64_t)Hkv * S;
+  const int64_t P = active_waves(T, a.n_waves);
+  const int wave = uniform(tid >> 6);
+  const int64_t w = (int64_t)blockIdx.x * kWavesPerWG + wave;
+  if (w >= P || T == 0) return;
+  const int64_t c0 = range_begin(w, T, P), c1 = range_begin(w + 1, T, P);
+  if (c0 >= c1) return;
+
+  // position: sequence s, kv head, tile, chunk k of n
+  int s = nvk_last_le(s_cs, a.batch, Hkv, c0, lane);
+  Seq sq = seq_of(a, s);
+  int n = uniform(chunks_of(sq)), tiles = uniform(tiles_of(a, sq));
+  int kvh, tile, k;
+  {
+    int64_t rr = c0 - (int64_t)Hkv * s_cs[s];
+    kvh = uniform((int)(rr / ((int64_t)tiles * n)));
+    rr -= (int64_t)kvh * tiles * n;
+    tile = uniform((int)(rr / n));
+    k = uniform((int)(rr % n));
+  }
+  bool started_here = k == 0;
+
+  const uint32_t buf0 = (uint32_t)uniform((int)(uint32_t)(size_t)(lds_ptr)(lds + wave * 2 * kBuf));
+  // ds_read_b64_tr_b4: the 16 lanes of group g read 8 bytes (16 dimensions) of keys 16 g .. +15;
+  // 16-byte chunks of a row are XOR-swizzled by its number so that they spread over the banks.
+  const int sw = HD == 128 ? (r >> 2) & 3 : (r >> 3) & 1;
+  const uint32_t tr_row = (uint32_t)((16 * g + r) * RB);
+  // DMA source of load j, lane l: bytes 16 (l % kCh) ^ swizzle of row (1024 / RB) j + l / kCh
+  constexpr int kCh = RB / 16, kRowsPerLoad = 1024 / RB;
+  const int vrow = lane / kCh;
+  const int vsw = HD == 128 ? (vrow >> 2) & 3 : (vrow >> 3) & 1;
+  const int vbyte = 16 * ((lane % kCh) ^ vsw);
+  // scale DMA: tensor, group and 8 keys of this lane (D = 64: both halves of the wave the same)
+  const int sl = HD == 128 ? lane : lane & 31;
+  const bool s_is_v = sl >= 32 * NG / 4;
+  const int s_grp = (sl >> 3) & (NG - 1), s_key = 8 * (sl & 7);
+
+  // Where a chunk lies: the index of its (16-key blocks') first row, and of the same row's scale.
+  struct Where {
+    int64_t row[kBlk], srow[kBlk];
+  };
+  auto locate = [&](const Seq& x, int ss, int hh, int kk) {
+    Where p;
+    const const_i32* bt = (const_i32*)(a.block_tables + (int64_t)ss * a.bt_stride);
+#pragma unroll
+    for (int b = 0; b < kBlk; ++b) {
+      int key = kk * kCK + 16 * b;
+      if (key >= x.keys) key = kk * kCK;  // a block past the keys: any block, nothing of it counts
+      const int logical = key / a.block_size;
+      int page = bt[logical];
+      if (page < 0 || page >= a.num_blocks) page = 0;
+      const int64_t head = (int64_t)page * Hkv + hh;
+      const int off = key - logical * a.block_size;
+      p.row[b] = head * a.block_size + off;
+      p.srow[b] = head * NG * a.block_size + off;
+    }
+    return p;
+  };
+  auto pick = [](const int64_t* v, int i) {  // v[i] of a lane's block i
+    if constexpr (kBlk == 1) return v[0];
+    else return i & 2 ? (i & 1 ? v[3] : v[2]) : (i & 1 ? v[1] : v[0]);
+  };
+  auto issue = [&](const Where& p, uint32_t buf, kvec (&kraw)[4]) {
+    const int64_t krow = kBlk == 1 ? p.row[0] + 16 * (r >> 2) : pick(p.row, r >> 2);
+    const uint8_t* kp = a.k_data + (krow + (r & 3)) * RB + g * (RB / 4);
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+      kraw[b] = __builtin_nontemporal_load(reinterpret_cast<const kvec*>(kp + 4 * b * RB));
+#pragma unroll
+    for (int j = 0; j < kVBytes / 1024; ++j) {
+      const int row = kRowsPerLoad * j + vrow;  // of the chunk
+      const int64_t vr = kBlk == 1 ? p.row[0] + row : pick(p.row, row >> 4) + (row & 15);
+      lds_load(a.v_data + vr * RB + vbyte, buf + 1024 * j);
+    }
+    const int64_t sr = kBlk == 1 ? p.srow[0] + s_key : pick(p.srow, s_key >> 4) + (s_key & 15);
+    lds_load((s_is_v ? a.v_scale : a.k_scale) + sr + (int64_t)s_grp * a.block_size, buf + kVBytes);
+  };
+
+  // per-group state
+  vec8 qf[NG];
+  nvk_f32x4 acc[HD / 16];
+  float m_run = -INFINITY, l_part = 0.f;
+  int tok = 0, head = 0, row_limit = 0, full_limit = 0;
+  bool row_valid = false;
+  auto start_group = [&]() {
+    const int rr = tile * kR + r;
+    tok = rr / a.G;
+    head = kvh * a.G + rr - tok * a.G;
+    row_valid = tok < sq.queries;
+    const int diag = sq.raw_keys - sq.queries;
+    row_limit = row_valid ? min(sq.keys - 1, diag + tok) : -1;           // last visible key
+    full_limit = uniform(min(sq.keys - 1, diag + tile * kR / a.G));      // visible to every row
+    const uint16_t* qp = a.q + (int64_t)(sq.row0 + tok) * a.q_stride_tok +
+                         (int64_t)head * a.q_stride_head + 8 * g;
+#pragma unroll
+    for (int i = 0; i < NG; ++i) {
+      nvk_u32x4 v = {0u, 0u, 0u, 0u};
+      if (row_valid) v = *reinterpret_cast<const nvk_u32x4*>(qp + 32 * i);
+      qf[i] = __builtin_bit_cast(vec8, v);
+    }
+#pragma unroll
+    for (int d = 0; d < HD / 16; ++d) acc[d] = nvk_f32x4{0.f, 0.f, 0.f, 0.f};
+    m_run = -INFINITY;
+    l_part = 0.f;
+  };
+
+  kvec kraw[4];
+  issue(locate(sq, s, kvh, k), buf0, kraw);
+  start_group();
+  uint32_t cur = 0;
+
+  for (int64_t c = c0;; ++c) {
+    // ---- the next chunk's position
+    const bool last = c + 1 == c1;
+    const bool group_end = k == n - 1;
+    int ns = s, nkvh = kvh, ntile = tile, nk = k + 1, nn = n, ntiles = tiles;
+    Seq nsq = sq;
+    if (group_end) {
+      nk = 0;
+      if (++ntile == tiles) {
+        ntile = 0;
+        if (++nkvh == Hkv) {
+          nkvh = 0;
+          if (!last) {
+            int b = s + 1;
+            while (s_cs[b + 1] == s_cs[b]) ++b;  // a next chunk exists
+            ns = uniform(b);
+            nsq = seq_of(a, ns);
+            nn = uniform(chunks_of(nsq));
+            ntiles = uniform(tiles_of(a, nsq));
+          }
+        }
+      }
+    }
+    Where np;
+    if (!last) np = locate(nsq, ns, nkvh, nk);
+
+    wait_all();
+    const uint32_t buf = buf0 + cur * kBuf;
+    kvec knext[4];
+    if (!last) issue(np, buf0 + (cur ^ 1) * kBuf, knext);
+
+    // ---- scores of keys 16 g + 4 b + i, row r
+    const int kbase = k * kCK;
+    nvk_f32x4 sc[4] = {};
+#pragma unroll
+    for (int i = 0; i < NG; ++i) {
+      const auto* sp = (const __attribute__((address_space(3))) nvk_f16x8*)(size_t)(
+          buf + kVBytes + 128 * i + 32 * g);
+      const nvk_f16x8 ks[2] = {sp[0], sp[1]};
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        const nvk_f32x4 z = {0.f, 0.f, 0.f, 0.f};
+        const nvk_f32x4 t = E::mfma16x16x32(fp4_unpack<F16>(kraw[b][i]), qf[i], z);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          sc[b][e] = fmaf(t[e], (float)ks[b >> 1][4 * (b & 1) + e], sc[b][e]);
+      }
+    }
+
+    // ---- mask, running maximum, probabilities
+    const bool full = kbase + kCK - 1 <= full_limit;
+    const int seen = row_limit - kbase - 16 * g + 1;  // of this lane's 16 keys, the first `seen`
+    if (!full) {
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sc[b][e] = 4 * b + e < seen ? sc[b][e] : -INFINITY;
+    }
+    float mx = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3]));
+#pragma unroll
+    for (int b = 1; b < 4; ++b)
+      mx = fmaxf(mx, fmaxf(fmaxf(sc[b][0], sc[b][1]), fmaxf(sc[b][2], sc[b][3])));
+    mx = nvk_max_xor32(max_xor16(mx));
+    const float m_new = fmaxf(m_run, mx == -INFINITY ? -INFINITY : mx * a.scale_log2);
+    const float moff = m_new == -INFINITY ? 0.f : m_new;
+    if (__builtin_amdgcn_ballot_w64(m_new > m_run)) {
+      const float alpha = nvk_fast_exp2(m_run - moff);  // 0 while nothing was visible
+      l_part *= alpha;
+#pragma unroll
+      for (int d = 0; d < HD / 16; ++d) acc[d] *= alpha;
+      m_run = m_new;
+    }
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        sc[b][e] = nvk_fast_exp2(fmaf(sc[b][e], a.scale_log2, -moff));
+        l_part += sc[b][e];
+      }
+
+    // ---- O^T += V^T (P vs)^T, one operand per group of dimensions
+    auto pv = [&](auto masked) {
+#pragma unroll
+      for (int i = 0; i < NG; ++i) {
+        const auto* sp = (const __attribute__((address_space(3))) nvk_f16x8*)(size_t)(
+            buf + kVBytes + 128 * NG + 128 * i + 32 * g);
+        nvk_f16x8 pf[2] = {sp[0], sp[1]};
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int j = 4 * (b & 1) + e;
+            const float x = sc[b][e] * (float)pf[b >> 1][j];
+            // a masked key's scale may be anything, what an earlier owner of the page left too
+            pf[b >> 1][j] = (_Float16)(!decltype(masked)::value || 4 * b + e < seen ? x : 0.f);
+          }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int d = 2 * i + h;
+          const i32x2 vc = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
+              (__attribute__((address_space(3))) i32x2*)(size_t)(buf + tr_row + 16 * (i ^ sw) +
+                                                                  8 * h));
+          acc[d] = NvkElt<true>::mfma16x16x32(fp4_unpack<true>((uint32_t)vc[0]), pf[0], acc[d]);
+          acc[d] = NvkElt<true>::mfma16x16x32(fp4_unpack<true>((uint32_t)vc[1]), pf[1], acc[d]);
+        }
+      }
+    };
+    if (full) pv(std::false_type{});
+    else pv(std::true_type{});
+
+    // ---- the group's or the range's end
+    if (group_end || last) {
+      const float l_tot = nvk_sum_xor32(sum_xor16(l_part));
+      if (group_end && started_here) {
+        if (row_valid) {
+          const float inv = l_tot == 0.f ? 0.f : 1.f / l_tot;
+          uint16_t* op = a.out + (int64_t)(sq.row0 + tok) * a.out_stride_tok +
+                         (int64_t)head * a.out_stride_head + 4 * g;
+#pragma unroll
+          for (int d = 0; d < HD / 16; ++d) {
+            nvk_u32x2 wv;
+            wv.x = E::pack2(acc[d][0] * inv, acc[d][1] * inv);
+            wv.y = E::pack2(acc[d][2] * inv, acc[d][3] * inv);
+            *reinterpret_cast<nvk_u32x2*>(op + 16 * d) = wv;
+          }
+        }
+      } else if (row_valid) {  // the merge reads the valid rows only
+        float* rec = a.rec + ((w * 2 + (started_here ? 0 : 1)) * a.rec_rows + r) * (int64_t)kRec;
+#pragma unroll
+        for (int d = 0; d < HD / 16; ++d)
+          *reinterpret_cast<nvk_f32x4*>(rec + 16 * d + 4 * g) = acc[d];
+        if (g == 0) {
+          rec[HD] = m_run;
+          rec[HD + 1] = l_tot;
+        }
+      }
+      if (lane == 0) {
+        const int64_t first = (int64_t)Hkv * s_cs[s] + ((int64_t)kvh * tiles + tile) * n;
+        const int p1 = (int)chunk_owner(first, T, P), p2 = (int)chunk_owner(first + n - 1, T, P);
+        const int64_t e = ((int64_t)s * Hkv + kvh) * a.max_tiles + tile;
+        *reinterpret_cast<int2*>(a.desc + 2 * e) = make_int2(p1, p2);
+      }
+      if (last) return;
+      s = ns;
+      sq = nsq;
+      kvh = uniform(nkvh);
+      tile = uniform(ntile);
+      n = nn;
+      tiles = ntiles;
+      k = 0;
+      started_here = true;
+      start_group();
+    } else {
+      k = uniform(nk);
+    }
+#pragma unroll
+    for (int b = 0; b < 4; ++b) kraw[b] = knext[b];
+    cur ^= 1;
+  }
+}
+
+// Merges the records of groups cut between waves and writes the rows of groups without a key.
+// grid = (Hkv * max_tiles * row pairs of a tile, batch), W waves: a workgroup owns two rows of a group
+// (HD / 4 lanes each, HD 64: half of them idle), wave v folds parts p1 + v, p1 + v + W, ... and wave 0
+// joins the waves' states through LDS.
+template <int HD, bool F16, int W>
+__global__ __launch_bounds__(64 * W) void fp4_merge_kernel(AttnArgs a) {
+  using E = NvkElt<F16>;
+  constexpr int kRec = HD + 4, kLanes = HD / 4, kBatch = 8;
+  const int pairs = (a.rec_rows + 1) / 2;
+  const int pair = blockIdx.x % pairs;
+  const int tile = blockIdx.x / pairs % a.max_tiles;
+  const int kvh = blockIdx.x / pairs / a.max_tiles;
+  const int s = blockIdx.y;
+  const int lane = threadIdx.x & 63, v = uniform(threadIdx.x >> 6);
+  const Seq sq = seq_of(a, s);
+  const int rows = min(sq.queries * a.G - tile * kR, a.rec_rows);  // of this tile
+  if (2 * pair >= rows) return;
+  const int64_t e = ((int64_t)s * a.num_kv_heads + kvh) * a.max_tiles + tile;
+  const int2 desc = *reinterpret_cast<const int2*>(a.desc + 2 * e);
+  const int p1 = desc.x, p2 = desc.y;
+  if (p1 >= 0 && p1 == p2) return;  // finished by one wave
+  const int half = lane / kLanes, d0 = 4 * (lane % kLanes);
+  const bool ok = half < 2 && 2 * pair + half < rows;
+  const int row = ok ? 2 * pair + half : 2 * pair;
+  float M = -INFINITY, L = 0.f;
+  nvk_f32x4 O = {0.f, 0.f, 0.f, 0.f};
+  if (p1 >= 0) {
+    for (int base = p1 + v; base <= p2; base += kBatch * W) {
+      float mv[kBatch], lv[kBatch];
+      nvk_f32x4 ov[kBatch];
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        const int p = base + u * W;
+        mv[u] = -INFINITY;
+        lv[u] = 0.f;
+        ov[u] = nvk_f32x4{0.f, 0.f, 0.f, 0.f};
+        if (p <= p2) {
+          const float* rec =
+              a.rec + (((int64_t)p * 2 + (p == p1 ? 0 : 1)) * a.rec_rows + row) * kRec;
+          mv[u] = rec[HD];
+          lv[u] = rec[HD + 1];
+          ov[u] = *reinterpret_cast<const nvk_f32x4*>(rec + d0);
+        }
+      }
+      float mb = M;
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) mb = fmaxf(mb, mv[u]);
+      const float mref = mb == -INFINITY ? 0.f : mb;
+      const float rs = nvk_fast_exp2(M - mref);
+      L *= rs;
+      O *= rs;
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        const float wt = nvk_fast_exp2(mv[u] - mref);
+        L += lv[u] * wt;
+        O += wt * ov[u];
+      }
+      M = mb;
+    }
+  }
+  if constexpr (W > 1) {
+    __shared__ float sm[W][64], sl[W][64];
+    __shared__ nvk_f32x4 so[W][64];
+    sm[v][lane] = M;
+    sl[v][lane] = L;
+    so[v][lane] = O;
+    __syncthreads();
+    if (v != 0) return;
+    float mx = M;
+#pragma unroll
+    for (int i = 1; i < W; ++i) mx = fmaxf(mx, sm[i][lane]);
+    const float mref = mx == -INFINITY ? 0.f : mx;
+    L = 0.f;
+    O = nvk_f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      const float wt = nvk_fast_exp2(sm[i][lane] - mref);
+      L += sl[i][lane] * wt;
+      O += wt * so[i][lane];
+    }
+  }
+  if (!ok) return;
+  const int rr = tile * kR + row;
+  const int tok = rr / a.G, head = kvh * a.G + rr - tok * a.G;
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  nvk_u32x2 wv;
+  wv.x = E::pack2(O[0] * inv, O[1] * inv);
+  wv.y = E::pack2(O[2] * inv, O[3] * inv);
+  *reinterpret_cast<nvk_u32x2*>(a.out + (int64_t)(sq.row0 + tok) * a.out_stride_tok +
+                                (int64_t)head * a.out_stride_head + d0) = wv;
+}
+
+// Sizes that follow from a call's static bounds.
+struct Plan {
+  int max_tiles, rec_rows, n_waves;
+  size_t desc_bytes, bytes;
+};
+bool plan_of(int batch, int max_queries, int num_q_heads, int num_kv_heads, int head_dim,
+             int block_size, int max_blocks, Plan& p) {
+  if (batch <= 0 || batch > kMaxBatch || max_queries <= 0 || num_q_heads <= 0 ||
+      num_kv_heads <= 0 || num_q_heads % num_kv_heads || block_size <= 0 || max_blocks <= 0)
+    return false;
+  if ((head_dim != 128 && head_dim != 64) || block_size % 16) return false;
+  const int G = num_q_heads / num_kv_heads;
+  if (G > kR) return false;
+  const int64_t rows = (int64_t)max_queries * G;
+  const int64_t chunks = ((int64_t)max_blocks * block_size + kCK - 1) / kCK;
+  const int64_t tiles = (rows + kR - 1) / kR;
+  if (tiles * num_kv_heads * 8 > INT32_MAX || chunks > INT32_MAX / kCK ||
+      tiles * chunks > INT32_MAX / batch || tiles * num_kv_heads > INT32_MAX / batch)
+    return false;
+  p.max_tiles = (int)tiles;
+  p.rec_rows = (int)(rows < kR ? rows : kR);
+  const int64_t units = tiles * chunks * batch * num_kv_heads;
+  int64_t wgs = (units + kWavesPerWG - 1) / kWavesPerWG;
+  if (wgs > kMaxWGs) wgs = kMaxWGs;
+  p.n_waves = (int)wgs * kWavesPerWG;
+  p.desc_bytes = ((size_t)batch * num_kv_heads * tiles * 8 + 255) / 256 * 256;
+  p.bytes = p.desc_bytes + (size_t)p.n_waves * 2 * p.rec_rows * (head_dim + 4) * sizeof(float);
+  return true;
+}
+
+template <int HD, bool F16>
+int launch(const AttnArgs& a, hipStream_t s) {
+  const dim3 grid(a.n_waves / kWavesPerWG), block(64 * kWavesPerWG);
+  if (a.block_size % kCK == 0)
+    hipLaunchKernelGGL((fp4_attention_kernel<HD, F16, true>), grid, block, 0, s, a);
+  else
+    hipLaunchKernelGGL((fp4_attention_kernel<HD, F16, false>), grid, block, 0, s, a);
+  const int st = nvk_launch_status();
+  if (st != NVK_OK) return st;
+  const dim3 mgrid(a.num_kv_heads * a.max_tiles * ((a.rec_rows + 1) / 2), a.batch);
+  // 32 waves and more per group: its parts are folded by 16 waves
+  if (a.n_waves >= 32 * (int64_t)a.batch * a.num_kv_heads * a.max_tiles)
+    hipLaunchKernelGGL((fp4_merge_kernel<HD, F16, 16>), mgrid, dim3(64 * 16), 0, s, a);
+  else
+    hipLaunchKernelGGL((fp4_merge_kernel<HD, F16, 1>), mgrid, dim3(64), 0, s, a);
+  return nvk_launch_status();
+}
+
+}  // namespace
+
+extern "C" size_t nvk_fp4_attention_workspace_size(int32_t batch, int32_t max_seqlen_q,
+                                                   int32_t num_q_heads, int32_t num_kv_heads,
+                                                   int32_t head_dim, int32_t block_size,
+                                                   int32_t max_blocks) {
+  Plan p;
+  return plan_of(batch, max_seqlen_q, num_q_heads, num_kv_heads, head_dim, block_size, max_blocks, p)
+             ? p.bytes
+             : 0;
+}
+
+extern "C" int nvk_fp4_attention(const void* q, int64_t q_stride_tok, int64_t q_stride_head,
+                                 int64_t total_q, const void* k_data, const void* k_scale,
+                                 const void* v_data, const void* v_scale,
+                                 const int32_t* cu_seqlens_q, const int32_t* seqlens_k,
+                                 int32_t batch, int32_t max_seqlen_q, const int32_t* block_tables,
+                                 int64_t bt_stride, int32_t max_blocks, int32_t block_size,
+                                 int32_t num_blocks, int32_t num_q_heads, int32_t num_kv_heads,
+                                 int32_t head_dim, float scale, void* out, int64_t out_stride_tok,
+                                 int64_t out_stride_head, void* workspace, size_t workspace_bytes,
+                                 int32_t dtype, void* stream) {
+  if (batch < 0 || total_q < 0 || max_seqlen_q < 0 || num_q_heads <= 0 || num_kv_heads <= 0 ||
+      block_size <= 0 || max_blocks < 0 || num_blocks < 0 || num_q_heads % num_kv_heads)
+    return NVK_EINVAL;
+  if (!(scale > 0.f)) return NVK_EINVAL;
+  if (dtype != NVK_DTYPE_BF16 && dtype != NVK_DTYPE_F16) return NVK_EUNSUPPORTED;
+  if (batch == 0 || total_q == 0 || max_seqlen_q == 0) return NVK_OK;
+  if (total_q > INT32_MAX) return NVK_EINVAL;
+  if (!cu_seqlens_q && (int64_t)batch * max_seqlen_q != total_q) return NVK_EINVAL;
+  Plan p;
+  if (num_blocks == 0 || !plan_of(batch, max_seqlen_q, num_q_heads, num_kv_heads, head_dim,
+                                  block_size, max_blocks, p))
+    return NVK_EUNSUPPORTED;
+  if (!q || !k_data || !k_scale || !v_data || !v_scale || !seqlens_k || !block_tables || !out)
+    return NVK_EINVAL;
+  if (bt_stride < max_blocks) return NVK_EINVAL;
+  if (((uintptr_t)q | (uintptr_t)k_data | (uintptr_t)k_scale | (uintptr_t)v_data |
+       (uintptr_t)v_scale) % 16 || q_stride_tok % 8 || q_stride_head % 8)
+    return NVK_EALIGN;
+  if ((uintptr_t)out % 8 || out_stride_tok % 4 || out_stride_head % 4) return NVK_EALIGN;
+  if (((uintptr_t)cu_seqlens_q | (uintptr_t)seqlens_k | (uintptr_t)block_tables) % 4)
+    return NVK_EALIGN;
+  if (!workspace || workspace_bytes < p.bytes) return NVK_EWORKSPACE;
+  if ((uintptr_t)workspace % 256) return NVK_EALIGN;
+  AttnArgs a{};
+  a.q = static_cast<const uint16_t*>(q);
+  a.q_stride_tok = q_stride_tok;
+  a.q_stride_head = q_stride_head;
+  a.total_q = total_q;
+  a.k_data = static_cast<const uint8_t*>(k_data);
+  a.k_scale = static_cast<const uint16_t*>(k_scale);
+  a.v_data = static_cast<const uint8_t*>(v_data);
+  a.v_scale = static_cast<const uint16_t*>(v_scale);
+  a.cu_q = cu_seqlens_q;
+  a.keys = seqlens_k;
+  a.block_tables = block_tables;
+  a.bt_stride = bt_stride;
+  a.batch = batch;
+  a.n_query = max_seqlen_q;
+  a.max_tiles = p.max_tiles;
+  a.cap = max_blocks * block_size;
+  a.block_size = block_size;
+  a.num_blocks = num_blocks;
+  a.num_kv_heads = num_kv_heads;
+  a.G = num_q_heads / num_kv_heads;
+  a.scale_log2 = scale * NVK_LOG2E;
+  a.out = static_cast<uint16_t*>(out);
+  a.out_stride_tok = out_stride_tok;
+  a.out_stride_head = out_stride_head;
+  a.desc = static_cast<int32_t*>(workspace);
+  a.rec = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.desc_bytes);
+  a.rec_rows = p.rec_rows;
+  a.n_waves = p.n_waves;
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  const bool f16 = dtype == NVK_DTYPE_F16;
+  if (head_dim == 128) return f16 ? launch<128, true>(a, s) : launch<128, false>(a, s);
+  return f16 ? launch<64, true>(a, s) : launch<64, false>(a, s);
+}

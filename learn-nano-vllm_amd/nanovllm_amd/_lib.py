@@ -99,6 +99,19 @@ SIGNATURES = {
     "nvk_sample": (ctypes.c_int, [_c_ptr, _c_i64, _c_i32, _c_i32, _c_i32, _c_ptr, _c_ptr, _c_i64,
                                   ctypes.c_uint64, ctypes.c_uint64, _c_ptr, _c_ptr, ctypes.c_size_t,
                                   _c_ptr]),
+    "nvk_fp4_store": (ctypes.c_int, [_c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_ptr,
+                                     _c_ptr, _c_i64, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32,
+                                     _c_ptr]),
+    "nvk_fp4_load": (ctypes.c_int, [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_i32, _c_i32,
+                                    _c_i32, _c_i32, _c_ptr, _c_i64, _c_ptr, _c_i64, _c_i32,
+                                    _c_ptr]),
+    "nvk_fp4_attention_workspace_size": (ctypes.c_size_t, [_c_i32, _c_i32, _c_i32, _c_i32, _c_i32,
+                                                           _c_i32, _c_i32]),
+    "nvk_fp4_attention": (ctypes.c_int, [_c_ptr, _c_i64, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_ptr,
+                                         _c_ptr, _c_ptr, _c_ptr, _c_i32, _c_i32, _c_ptr, _c_i64,
+                                         _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32,
+                                         ctypes.c_float, _c_ptr, _c_i64, _c_i64, _c_ptr,
+                                         ctypes.c_size_t, _c_i32, _c_ptr]),
     "nvk_gather_last_tokens": (ctypes.c_int, [_c_ptr, _c_i64, _c_ptr, _c_i32, _c_i32, _c_i32, _c_ptr,
                                               _c_i64, _c_ptr]),
 }
@@ -172,6 +185,13 @@ def on_device(device: torch.device):
     """``torch.cuda.device(device)``, or nothing where it is current already."""
     current = device.index is None or device.index == torch.cuda.current_device()
     return _NO_SWITCH if current else torch.cuda.device(device)
+
+
+def int32(t: torch.Tensor) -> torch.Tensor:
+    """`t` as a contiguous int32 tensor."""
+    if t.dtype != torch.int32:
+        t = t.to(torch.int32)
+    return t.contiguous()
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

@@ -13,6 +13,7 @@ from __future__ import annotations
 import torch
 
 from nanovllm_amd import _lib
+from nanovllm_amd.fp4_cache import Fp4Cache, fp4_attention
 
 
 def _unsupported(**opts) -> None:
@@ -32,10 +33,7 @@ def _attn_dtype(*ts: torch.Tensor) -> int:
     return _lib.dtype_code(ts[0])
 
 
-def _int32(t: torch.Tensor) -> torch.Tensor:
-    if t.dtype != torch.int32:
-        t = t.to(torch.int32)
-    return t.contiguous()
+_int32 = _lib.int32
 
 
 def _key_bound(k, block_table, max_seqlen_k):
@@ -81,7 +79,13 @@ def varlen_prefill(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, softmax_sc
     library uses it to decide whether to split long key ranges across
     workgroups (its workspace is this stream's cached buffer).  ``order``:
     from prefill_tile_order with the same metadata (ranked once per step).
+    k and v may be ``Fp4Cache`` (paged, with ``block_table``); ``order`` is then unused.
     """
+    if isinstance(k, Fp4Cache) or isinstance(v, Fp4Cache):
+        if block_table is None:
+            raise _lib.NvkError("a 4-bit cache is read through a block_table")
+        return fp4_attention(q, k, v, cu_seqlens_k, block_table, softmax_scale,
+                             cu_seqlens_q=cu_seqlens_q, max_seqlen_q=max_seqlen_q, out=out)
     dev = _lib.require_gpu(q, k, v, cu_seqlens_q, cu_seqlens_k, block_table)
     dtype = _attn_dtype(q, k, v)
     if q.dim() != 3 or q.stride(-1) != 1:
@@ -149,7 +153,10 @@ def varlen_prefill(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, softmax_sc
 
 def paged_decode(q, k_cache, v_cache, context_lens, block_table, softmax_scale, out=None):
     """One query per sequence over its paged cache.  q: [B, Hq, D] (any token /
-    head strides).  Returns [B, Hq, D] (or fills ``out``)."""
+    head strides).  Returns [B, Hq, D] (or fills ``out``).  The caches may be
+    ``Fp4Cache``."""
+    if isinstance(k_cache, Fp4Cache) or isinstance(v_cache, Fp4Cache):
+        return fp4_attention(q, k_cache, v_cache, context_lens, block_table, softmax_scale, out=out)
     dev = _lib.require_gpu(q, k_cache, v_cache, context_lens, block_table)
     dtype = _attn_dtype(q, k_cache, v_cache)
     if q.dim() != 3 or q.stride(-1) != 1:
@@ -239,7 +246,7 @@ def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, rotary_cos=None
     speculative-decode verification) runs the causal varlen kernel with the
     query block aligned to the end of each sequence's cache_seqlens keys.
     Without block_table the caches are [B, S, Hkv, D]: sequence b is then one
-    page of S slots.
+    page of S slots.  The caches may be ``Fp4Cache``.
     """
     _unsupported(k=(k, None), v=(v, None), rotary_cos=(rotary_cos, None),
                  rotary_sin=(rotary_sin, None), cache_batch_idx=(cache_batch_idx, None),
@@ -249,7 +256,8 @@ def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, rotary_cos=None
     if q.dim() != 4:
         raise _lib.NvkError("q must be [batch, seqlen_q, heads, head_dim]")
     b, sq, hq, d = q.shape
-    dev = _lib.require_gpu(q, k_cache, v_cache)
+    fp4 = isinstance(k_cache, Fp4Cache) or isinstance(v_cache, Fp4Cache)
+    dev = _lib.require_gpu(q) if fp4 else _lib.require_gpu(q, k_cache, v_cache)
     if cache_seqlens is None:
         raise NotImplementedError("nanovllm_amd: cache_seqlens is required")
     if isinstance(cache_seqlens, int):
@@ -261,6 +269,10 @@ def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, rotary_cos=None
         return out.view(b, 1, hq, d)
     if not causal:
         raise NotImplementedError("nanovllm_amd: seqlen_q > 1 needs causal=True")
+    if fp4:
+        out = fp4_attention(q.reshape(b * sq, hq, d), k_cache, v_cache, cache_seqlens, block_table,
+                            softmax_scale, max_seqlen_q=sq)
+        return out.view(b, sq, hq, d)
     lens = _int32(cache_seqlens)
     out = _verify(q, k_cache, v_cache, lens, block_table, softmax_scale)
     if out is not None:

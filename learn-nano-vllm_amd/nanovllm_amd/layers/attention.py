@@ -10,6 +10,7 @@ import torch
 from torch import nn
 
 from nanovllm_amd import _lib
+from nanovllm_amd.fp4_cache import Fp4Cache, fp4_store
 from nanovllm_amd.flash_api import paged_decode, prefill_tile_order, varlen_prefill
 from nanovllm_amd.utils.context import get_context
 
@@ -21,7 +22,10 @@ def store_kvcache(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor,
     key/value: [N, num_kv_heads, head_dim]; each token row contiguous
     (row stride free: value is a view of the packed qkv).  Caches
     [num_blocks, block_size, num_kv_heads, head_dim]; slot -1 skips the token.
+    Into ``Fp4Cache`` caches the rows are quantised as they are stored.
     """
+    if isinstance(k_cache, Fp4Cache) or isinstance(v_cache, Fp4Cache):
+        return fp4_store(key, value, k_cache, v_cache, slot_mapping)
     N, num_heads, head_dim = key.shape
     D = num_heads * head_dim
     assert key.stride(-1) == 1 and value.stride(-1) == 1
@@ -80,6 +84,8 @@ class Attention(nn.Module):
     kv_stored=True (an addition; the reference has no such argument) skips the
     store because the fused prologue (layers/prologue.py) already wrote the
     caches; k may then be None unless the step is a dense prefill.
+    k_cache / v_cache may be ``Fp4Cache``: new keys and values are then quantised
+    as they are stored, and a step with block tables reads what the caches hold.
     """
 
     def __init__(self, num_heads, head_dim, scale, num_kv_heads):
@@ -98,7 +104,9 @@ class Attention(nn.Module):
         if context.is_prefill:
             if context.block_tables is not None:    # prefix cache / later chunk
                 k, v = k_cache, v_cache
-            order = _prefill_order(context, q, k, context.block_tables)
+            order = None
+            if not isinstance(k, Fp4Cache):
+                order = _prefill_order(context, q, k, context.block_tables)
             o = varlen_prefill(q, k, v, context.cu_seqlens_q, context.cu_seqlens_k,
                                context.max_seqlen_q, self.scale, block_table=context.block_tables,
                                max_seqlen_k=context.max_seqlen_k, order=order)

@@ -26,6 +26,7 @@ from __future__ import annotations
 import torch
 
 from nanovllm_amd import _lib
+from nanovllm_amd.fp4_cache import Fp4Cache
 from nanovllm_amd.flash_api import _int32, _key_bound
 from nanovllm_amd.layers.attention import Attention, _prefill_order
 from nanovllm_amd.utils.context import get_context
@@ -272,6 +273,12 @@ def attention_with_prologue(attn, positions: torch.Tensor, qkv: torch.Tensor, q_
     ``attn(q, k, v)`` returns ([T, Hq, D] prefill, [B, 1, Hq, D] decode)."""
     assert q_norm.eps == k_norm.eps    # one eps for both norms (qwen3.py:70-71)
     context = get_context()
+    if isinstance(attn.k_cache, Fp4Cache) or isinstance(attn.v_cache, Fp4Cache):
+        # norms and rotation, then the store that quantises and the attention
+        q, k, v = qk_norm_rope_store(positions, qkv, attn.num_heads, attn.num_kv_heads,
+                                     attn.head_dim, q_norm.weight, k_norm.weight, q_norm.eps,
+                                     rotary_emb.cos_sin_cache)
+        return attn(q, k, v)
     store = bool(attn.k_cache.numel() and attn.v_cache.numel())
     if (store and not context.is_prefill and attn.head_dim == 128
             and qkv.shape[0] <= FUSED_DECODE_MAX_BATCH):

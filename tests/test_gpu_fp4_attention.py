@@ -1,0 +1,282 @@
+"""Attention over the 4-bit cache on the GPU against the oracle in 64 bits, within bounds that follow
+from the types (oracle.fp4_oracle.attention)."""
+import numpy as np
+import pytest
+import torch
+
+from fp4_utils import DTYPES, Pages, assert_close, rng_rows, tables_of
+from gpu_utils import say
+from nanovllm_amd import (Fp4Cache, flash_attn_varlen_func, flash_attn_with_kvcache, paged_decode,
+                          varlen_prefill)
+from oracle import fp4_oracle as orc
+
+pytestmark = pytest.mark.gpu
+
+
+def _reference(q, pages, tables, n_queries, lens, scale):
+    """Oracle of sequences whose queries follow each other in q [tokens, Hq, D]."""
+    qn = q.double().cpu().numpy()
+    out, size = np.zeros(qn.shape), np.zeros(qn.shape)
+    at = 0
+    for b, (n, m) in enumerate(zip(n_queries, lens)):
+        k, v = pages.rows(tables[b], m)
+        out[at:at + n], size[at:at + n] = orc.attention(qn[at:at + n], k, v, m, scale)
+        at += n
+    return out, size
+
+
+def _int(a):
+    return torch.as_tensor(np.asarray(a, dtype=np.int32)).cuda()
+
+
+LADDER = [1, 0, 15, 16, 17, 63, 64, 65, 255, 256, 257, 1000]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("hq,hkv,d,bs", [(16, 8, 128, 256), (16, 16, 128, 64), (16, 4, 128, 256),
+                                         (16, 2, 128, 256), (12, 4, 128, 48), (16, 1, 128, 16),
+                                         (8, 4, 64, 256), (8, 1, 64, 16), (3, 1, 64, 32)])
+def test_decode_over_a_ladder_of_contexts(hq, hkv, d, bs, dtype):
+    tables, nb = tables_of(LADDER, bs, 1)
+    pages = Pages(5, nb, bs, hkv, d, dtype)
+    q = rng_rows(9, (len(LADDER), hq, d), dtype).cuda()
+    say(f"fp4 decode ladder {hq}/{hkv} x {d} pages {bs} {dtype}")
+    out = paged_decode(q, *pages.gpu(), _int(LADDER), _int(tables), d ** -0.5)
+    ref, size = _reference(q, pages, tables, [1] * len(LADDER), LADDER, d ** -0.5)
+    assert not out[1].any()                        # no key: zeros
+    assert_close(out, ref, size, dtype, "fp4 decode ladder")
+
+
+@pytest.mark.parametrize("lens", [[5000], [1500, 3000], [64], [2100] * 3 + [1] * 30])
+@pytest.mark.parametrize("bs", [256, 16])
+def test_decode_of_contexts_cut_into_many_parts(lens, bs):
+    tables, nb = tables_of(lens, bs, 2)
+    pages = Pages(6, nb, bs, 2, 128)
+    q = rng_rows(3, (len(lens), 4, 128), "bf16").cuda()
+    say(f"fp4 decode {lens[:4]} pages {bs}")
+    out = paged_decode(q, *pages.gpu(), _int(lens), _int(tables), None)
+    ref, size = _reference(q, pages, tables, [1] * len(lens), lens, 128 ** -0.5)
+    assert_close(out, ref, size, "bf16", "fp4 decode parts")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("n,hq,hkv,d", [(2, 16, 8, 128), (6, 16, 8, 128), (8, 16, 8, 128),
+                                        (5, 8, 1, 128), (33, 4, 2, 128), (3, 4, 4, 64),
+                                        (70, 2, 2, 64)])
+def test_several_queries_of_every_sequence(n, hq, hkv, d, dtype):
+    lens = [n, n + 1, 64, 300, 130, max(0, n - 1), 0]     # two with rows that see no key
+    tables, nb = tables_of(lens, 64, 4)
+    pages = Pages(7, nb, 64, hkv, d, dtype)
+    q = rng_rows(11, (len(lens), n, hq, d), dtype).cuda()
+    say(f"fp4 {n} queries {hq}/{hkv} x {d} {dtype}")
+    out = flash_attn_with_kvcache(q, *pages.gpu(), cache_seqlens=_int(lens),
+                                  block_table=_int(tables), causal=True)
+    ref, size = _reference(q.flatten(0, 1), pages, tables, [n] * len(lens), lens, d ** -0.5)
+    assert out.shape == q.shape
+    assert_close(out, ref, size, dtype, "fp4 several queries")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("bs", [256, 16])
+@pytest.mark.parametrize("news,cached", [([3, 0, 40, 1, 9], [0, 70, 5, 300, 64]),
+                                         ([200, 17], [100, 0]), ([1], [1])])
+def test_ragged_queries(news, cached, bs, dtype):
+    hq, hkv, d = 8, 4, 128
+    lens = [a + b for a, b in zip(news, cached)]
+    tables, nb = tables_of(lens, bs, 8)
+    pages = Pages(12, nb, bs, hkv, d, dtype)
+    total = sum(news)
+    # two rows behind the last sequence stay as they were
+    out = torch.full((total + 2, hq, d), 7.0, dtype=DTYPES[dtype], device="cuda")
+    q = rng_rows(13, (total + 2, hq, d), dtype).cuda()
+    cu = lambda v: _int(np.concatenate([[0], np.cumsum(v)]))
+    say(f"fp4 ragged {news} pages {bs} {dtype}")
+    varlen_prefill(q, *pages.gpu(), cu(news), cu(lens), max(news), None, block_table=_int(tables),
+                   out=out)
+    ref, size = _reference(q[:total], pages, tables, news, lens, d ** -0.5)
+    assert_close(out[:total], ref, size, dtype, "fp4 ragged")
+    assert (out[total:] == 7.0).all()
+    got = flash_attn_varlen_func(q, *pages.gpu(), cu(news), cu(lens), max(news), max(lens),
+                                 causal=True, block_table=_int(tables))
+    assert torch.equal(got[:total], out[:total])
+
+
+def test_queries_and_outputs_with_strides():
+    lens = [77, 130]
+    tables, nb = tables_of(lens, 64, 4)
+    pages = Pages(7, nb, 64, 2, 128)
+    wide = rng_rows(1, (2, 3, 4 * 128 + 64), "bf16").cuda()
+    q = wide[:, 1, 32:32 + 512].view(2, 4, 128)
+    buf = torch.full((2, 4, 160), 3.0, dtype=torch.bfloat16, device="cuda")
+    table = torch.full((2, 7), -1, dtype=torch.int64, device="cuda")
+    table[:, 1:1 + tables.shape[1]] = _int(tables)
+    paged_decode(q, *pages.gpu(), _int(lens).long(), table[:, 1:], 0.1, out=buf[:, :, 16:144])
+    ref, size = _reference(q, pages, tables, [1, 1], lens, 0.1)
+    assert_close(buf[:, :, 16:144], ref, size, "bf16", "fp4 strides")
+    assert (buf[:, :, :16] == 3.0).all() and (buf[:, :, 144:] == 3.0).all()
+
+
+def test_what_lies_past_a_context_or_behind_the_mask_does_not_count():
+    """NaN and infinite scales in a page's slots past the context, and NaN in a key that only the
+    later query sees."""
+    lens, n = [40, 100], 2
+    tables, nb = tables_of(lens, 64, 4)
+    pages = Pages(7, nb, 64, 2, 128)
+    q = rng_rows(1, (2, n, 4, 128), "bf16").cuda()
+    ref, size = _reference(q.flatten(0, 1), pages, tables, [n, n], lens, 128 ** -0.5)
+    for i in range(2):
+        for b, m in enumerate(lens):
+            page, off = tables[b][(m - 1) // 64], (m - 1) % 64
+            pages.np[i][1][page, :, :, off + 1:] = np.nan if b else np.inf
+            pages.np[i][0][page, :, off + 1:] = 0xFF
+            pages.np[i][1][page, 0, :, off] = np.nan     # the last key of head 0
+    out = flash_attn_with_kvcache(q, *pages.gpu(), cache_seqlens=_int(lens),
+                                  block_table=_int(tables), causal=True).cpu()
+    assert torch.isnan(out[:, 1, :2]).all()          # the query that sees it, heads of kv head 0
+    keep = np.ones((2, n, 4), bool)
+    keep[:, 1, :2] = False
+    ref, size = ref.reshape(2, n, 4, 128), size.reshape(2, n, 4, 128)
+    assert_close(out[torch.from_numpy(keep)], ref[keep], size[keep], "bf16", "fp4 masked NaN")
+
+
+def test_a_value_that_is_not_finite_stays_in_its_dimensions():
+    lens = [130]
+    tables, nb = tables_of(lens, 64, 4)
+    pages = Pages(7, nb, 64, 1, 128)
+    ref, size = _reference(rng_rows(1, (1, 2, 128), "bf16"), pages, tables, [1], lens, 128 ** -0.5)
+    pages.np[1][1][tables[0][1], 0, 2, 5] = np.nan     # group 2 of one token's value
+    out = paged_decode(rng_rows(1, (1, 2, 128), "bf16").cuda(), *pages.gpu(), _int(lens),
+                       _int(tables), None).cpu()
+    assert torch.isnan(out[..., 64:96]).all()
+    keep = [d for d in range(128) if not 64 <= d < 96]
+    assert_close(out[..., keep], ref[..., keep], size[..., keep], "bf16", "fp4 NaN value")
+
+
+def test_scores_far_apart_and_scales_of_many_magnitudes():
+    """One key far above the others, values from 1e-3 to 1e3: the running maximum moves late."""
+    n, hkv, d = 700, 2, 128
+    rows_k = rng_rows(1, (n, hkv, d), "bf16").double().numpy()
+    rows_k[650] *= 60
+    rows_k[10] *= -40
+    rows_v = rng_rows(2, (n, hkv, d), "bf16", spread=1e3).double().numpy()
+    nb, bs = 11, 64
+    pages = Pages(3, nb, bs, hkv, d)
+    for i, rows in enumerate((rows_k, rows_v)):
+        orc.store(rows, *pages.np[i], np.arange(n), i == 0)
+    q = rng_rows(5, (1, 4, d), "bf16").cuda()
+    out = paged_decode(q, *pages.gpu(), _int([n]), _int([np.arange(nb)]), None)
+    ref, size = _reference(q, pages, [np.arange(nb)], [1], [n], d ** -0.5)
+    assert_close(out, ref, size, "bf16", "fp4 far scores")
+
+
+def test_page_ids_outside_the_cache_are_not_followed():
+    lens = [100, 100, 100]
+    tables, nb = tables_of(lens, 64, 4)
+    pages = Pages(7, nb, 64, 2, 128)
+    q = rng_rows(1, (3, 4, 128), "bf16").cuda()
+    ref, size = _reference(q, pages, tables, [1] * 3, lens, 128 ** -0.5)
+    bad = tables.copy()
+    bad[1] = [nb, -7]
+    out = paged_decode(q, *pages.gpu(), _int(lens), _int(bad), None)
+    assert torch.isfinite(out).all()
+    for b in (0, 2):
+        assert_close(out[b], ref[b], size[b], "bf16", "fp4 beside a bad table")
+    # lengths beyond the table's pages are cut to them
+    out = paged_decode(q, *pages.gpu(), _int([10 ** 6] * 3), _int(tables), None)
+    full, fsize = _reference(q, pages, tables, [1] * 3, [128] * 3, 128 ** -0.5)
+    assert_close(out, full, fsize, "bf16", "fp4 lengths past the table")
+
+
+def test_without_a_block_table_every_sequence_is_a_page():
+    lens = [5, 48]
+    pages = Pages(7, 2, 48, 2, 128)
+    q = rng_rows(1, (2, 1, 4, 128), "bf16").cuda()
+    out = flash_attn_with_kvcache(q, *pages.gpu(), cache_seqlens=_int(lens), causal=True)
+    ref, size = _reference(q[:, 0], pages, [[0], [1]], [1, 1], lens, 128 ** -0.5)
+    assert_close(out[:, 0], ref, size, "bf16", "fp4 no table")
+    out = flash_attn_with_kvcache(q, *pages.gpu(), cache_seqlens=7, causal=True)
+    ref, size = _reference(q[:, 0], pages, [[0], [1]], [1, 1], [7, 7], 128 ** -0.5)
+    assert_close(out[:, 0], ref, size, "bf16", "fp4 int length")
+
+
+def test_pages_past_4_gib():
+    hkv, d, bs = 8, 128, 256
+    nb = (1 << 32) // (hkv * bs * d // 2) + 4
+    small = Pages(7, 4, bs, hkv, d)
+    kc, vc = Fp4Cache.zeros(nb, bs, hkv, d), Fp4Cache.zeros(nb, bs, hkv, d)
+    for c, s in zip((kc, vc), small.gpu()):
+        c.data[-4:], c.scale[-4:] = s.data, s.scale
+    lens = [1000, 3]
+    tables = np.array([[1, 3, 0, 2], [2, -1, -1, -1]], np.int32)
+    q = rng_rows(1, (2, 16, d), "bf16").cuda()
+    say("fp4 decode past 4 GiB")
+    out = paged_decode(q, kc, vc, _int(lens), _int(np.where(tables >= 0, tables + nb - 4, -1)), None)
+    ref, size = _reference(q, small, tables, [1, 1], lens, d ** -0.5)
+    assert_close(out, ref, size, "bf16", "fp4 past 4 GiB")
+
+
+def test_a_captured_decode_follows_its_inputs():
+    """A graph replayed with other lengths, tables and queries, eager calls between the replays."""
+    bs, hkv, hq, d = 256, 8, 16, 128
+    first = [300, 40, 0, 700]
+    tables, nb = tables_of([700] * 4, bs, 3)
+    pages = Pages(7, nb, bs, hkv, d)
+    kc, vc = pages.gpu()
+    q, lens, bt = rng_rows(1, (4, hq, d), "bf16").cuda(), _int(first), _int(tables)
+    paged_decode(q, kc, vc, lens, bt, None)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = paged_decode(q, kc, vc, lens, bt, None)
+    for i, now in enumerate([first, [1, 2, 3, 4], [700, 0, 256, 257], first]):
+        q.copy_(rng_rows(20 + i, (4, hq, d), "bf16"))
+        lens.copy_(_int(now))
+        graph.replay()
+        eager = paged_decode(q, kc, vc, lens, bt, None)
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager)
+        ref, size = _reference(q, pages, tables, [1] * 4, now, d ** -0.5)
+        assert_close(out, ref, size, "bf16", f"fp4 replay {i}")
+
+
+def test_two_streams_at_once():
+    lens = [900] * 8
+    tables, nb = tables_of(lens, 256, 3)
+    pages = Pages(7, nb, 256, 8, 128)
+    kc, vc = pages.gpu()
+    qs = [rng_rows(i, (8, 16, 128), "bf16").cuda() for i in range(2)]
+    args = (_int(lens), _int(tables), None)
+    want = [paged_decode(q, kc, vc, *args) for q in qs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in qs]
+    got = [[], []]
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(paged_decode(qs[i], kc, vc, *args))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(g, want[i]) for g in got[i])
+
+
+def test_refusals():
+    pages = Pages(7, 2, 64, 2, 128)
+    kc, vc = pages.gpu()
+    q = rng_rows(1, (2, 4, 128), "bf16").cuda()
+    lens, bt = _int([3, 4]), _int([[0], [1]])
+    for bad in (lambda: paged_decode(q, kc, vc, lens, bt[:1], None),
+                lambda: paged_decode(q, kc, vc, lens[:1], bt, None),
+                lambda: paged_decode(q[..., :64], kc, vc, lens, bt, None),
+                lambda: paged_decode(q.float(), kc, vc, lens, bt, None),
+                lambda: paged_decode(q[:, :3], kc, vc, lens, bt, None),
+                lambda: paged_decode(q, kc, vc, lens, bt, 0.0),
+                lambda: paged_decode(q, kc, vc, lens, bt, None, out=q.float()),
+                lambda: paged_decode(q, kc, pages.np[1], lens, bt, None),
+                lambda: varlen_prefill(q, kc, vc, _int([0, 2]), _int([0, 3, 4]), 2, None,
+                                       block_table=bt[:1])):
+        with pytest.raises(Exception) as e:
+            bad()
+        assert "Nvk" in type(e.value).__name__
+    with pytest.raises(NotImplementedError):
+        flash_attn_with_kvcache(q.view(1, 2, 4, 128), kc, vc, cache_seqlens=_int([3]),
+                                block_table=_int([[0]]))
