@@ -576,30 +576,36 @@ int nvk_fp4_load(const void* k_data, const void* k_scale, const void* v_data, co
  *
  * cu_seqlens_q == NULL: max_seqlen_q queries per sequence (total_q = batch * max_seqlen_q),
  *   seqlens_k [batch] its keys (context lengths, the queries' own tokens among them).
- * Otherwise both are prefix sums [batch + 1], as in nvk_varlen_prefill; queries past
- *   max_seqlen_q, and sequences that do not lie within q's total_q rows, are left unwritten.
+ * Otherwise both are prefix sums [batch + 1], as in nvk_varlen_prefill: no range of queries is longer
+ *   than max_seqlen_q, and their sum is at most total_q; rows behind it are left as they were.
+ * max_seqlen_k (0 = unknown) bounds the keys of a sequence, on the host: what a workspace for many
+ *   queries has to hold.
  * Query i of Lq sees key j iff j <= i + Lk - Lq; one that sees none is written as zeros.
  * q, out, block_tables, scale: as in nvk_paged_decode.  A page id outside [0, num_blocks) is never
  *   followed; the output of a sequence that names one is unspecified.
- * The scores are f32 sums of exact products; a probability times its value's scale is rounded to
- *   f16 before the product with the codes, whose sums are f32.
+ * Up to 128 rows (queries x G): the scores are f32 sums of exact products; a probability times its
+ *   value's scale is rounded to f16 before the product with the codes, whose sums are f32.
+ *   More rows, head_dim 128 and G 1, 2, 4 or 8: keys and values pass through f16 pages in the
+ *   workspace (512 MiB of them, or one sequence's if that is more; a larger batch goes in parts),
+ *   rounded once, f32 sums again.  There a query that sees a value that is not finite gets NaN in
+ *   all of its head, not only in that value's dimensions.
  * G = num_q_heads / num_kv_heads: at most 16.  batch <= 2048.
  * workspace: device scratch of nvk_fp4_attention_workspace_size() bytes, 256-byte aligned, not
  *   initialised; two calls in flight at once need two.  The size is 0 for sizes that are not
- *   supported (the call returns NVK_EUNSUPPORTED).  Two kernels.
+ *   supported (the call returns NVK_EUNSUPPORTED).
  */
-size_t nvk_fp4_attention_workspace_size(int32_t batch, int32_t max_seqlen_q, int32_t num_q_heads,
-                                        int32_t num_kv_heads, int32_t head_dim,
-                                        int32_t block_size, int32_t max_blocks);
+size_t nvk_fp4_attention_workspace_size(int32_t batch, int32_t max_seqlen_q, int32_t max_seqlen_k,
+                                        int32_t num_q_heads, int32_t num_kv_heads,
+                                        int32_t head_dim, int32_t block_size, int32_t max_blocks);
 int nvk_fp4_attention(const void* q, int64_t q_stride_tok, int64_t q_stride_head, int64_t total_q,
                       const void* k_data, const void* k_scale, const void* v_data,
                       const void* v_scale, const int32_t* cu_seqlens_q, const int32_t* seqlens_k,
-                      int32_t batch, int32_t max_seqlen_q, const int32_t* block_tables,
-                      int64_t bt_stride, int32_t max_blocks, int32_t block_size,
-                      int32_t num_blocks, int32_t num_q_heads, int32_t num_kv_heads,
-                      int32_t head_dim, float scale, void* out, int64_t out_stride_tok,
-                      int64_t out_stride_head, void* workspace, size_t workspace_bytes,
-                      int32_t dtype, void* stream);
+                      int32_t batch, int32_t max_seqlen_q, int32_t max_seqlen_k,
+                      const int32_t* block_tables, int64_t bt_stride, int32_t max_blocks,
+                      int32_t block_size, int32_t num_blocks, int32_t num_q_heads,
+                      int32_t num_kv_heads, int32_t head_dim, float scale, void* out,
+                      int64_t out_stride_tok, int64_t out_stride_head, void* workspace,
+                      size_t workspace_bytes, int32_t dtype, void* stream);
 
 #ifdef __cplusplus
 }

@@ -44,3 +44,41 @@ template <int HD, bool KEYS>
 NVK_DEVICE int fp4_place(int u) {
   return KEYS ? (HD / 32) * (u & 3) + (u >> 2) : u;
 }
+
+// ---- long query ranges: the pages in f16, and the prefill kernel over them --------------------------
+// A tile of 128 query rows reads every key 8 times less often than one of 16, and its matrix
+// instructions leave no time to convert the codes once per wave.  So a pass converts a step's
+// keys and values once, into pages of 256 tokens in the workspace, sequence after sequence.
+constexpr int kFp4Page = 256;
+// f16 pages of a bf16 model hold keys and values times 2^-3: 6 * 65504, the format's largest, fits.
+// (An f16 model's own are held as they are, the largest cut to 65504.)
+constexpr int kFp4KeyShift = 3;
+
+struct Fp4Expand {
+  const uint8_t *k_data, *v_data;
+  const uint16_t *k_scale, *v_scale;
+  const int32_t* block_tables;
+  int64_t bt_stride;
+  const int32_t* cu_k;
+  int batch, pages_per_seq, max_blocks, block_size, num_blocks, num_kv_heads;
+  uint16_t *k_pages, *v_pages;  // [batch * pages_per_seq][kFp4Page][num_kv_heads][128]
+  int32_t* tables;              // [batch][pages_per_seq]: the pages' numbers
+  bool f16;                     // of an f16 model
+};
+int fp4_expand_launch(const Fp4Expand& p, hipStream_t stream);
+
+// Varlen attention over such pages (varlen_prefill.hip); q and out are f16 or bf16.
+struct Fp4Prefill {
+  const void* q;
+  int64_t q_stride_tok, q_stride_head, total_q;
+  const void *k_pages, *v_pages;
+  const int32_t *cu_q, *cu_k, *tables;
+  int batch, max_seqlen_q, max_seqlen_k, pages_per_seq, num_q_heads, num_kv_heads;
+  float scale;
+  void* out;
+  int64_t out_stride_tok, out_stride_head;
+  void* workspace;
+  size_t workspace_bytes;
+  bool f16;
+};
+int fp4_prefill_launch(const Fp4Prefill& p, hipStream_t stream);

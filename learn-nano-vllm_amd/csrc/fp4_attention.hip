@@ -592,29 +592,143 @@ int launch(const AttnArgs& a, hipStream_t s) {
   return nvk_launch_status();
 }
 
+// Long query ranges go through f16 pages (fp4.h).
+#ifndef NVK_FP4_DIRECT_ROWS
+#define NVK_FP4_DIRECT_ROWS 128
+#endif
+constexpr int kDirectRows = NVK_FP4_DIRECT_ROWS;  // rows per kv head that the kernel above takes itself
+constexpr int64_t kPageBytesMost = (int64_t)512 << 20;  // pages of a part of the batch (one sequence: any)
+
+// Workspace of that route, for `part` sequences at a time.
+struct PagePlan {
+  int part, pages_per_seq, max_keys;
+  size_t cu_bytes, table_bytes, page_bytes, attn_bytes, bytes;  // page_bytes: of keys, and of values
+};
+bool page_plan(int batch, int max_queries, int max_seqlen_k, int num_q_heads, int num_kv_heads,
+               int head_dim, int block_size, int max_blocks, PagePlan& p) {
+  const int G = num_q_heads / num_kv_heads;
+  if (head_dim != 128 || (G != 1 && G != 2 && G != 4 && G != 8) ||
+      (int64_t)max_queries * G <= kDirectRows)
+    return false;
+  int64_t keys = (int64_t)max_blocks * block_size;
+  if (max_seqlen_k > 0 && max_seqlen_k < keys) keys = max_seqlen_k;
+  if ((int64_t)num_kv_heads * head_dim >= (1 << 23) ||
+      (int64_t)kFp4Page * num_kv_heads * head_dim * 2 > UINT32_MAX || num_kv_heads > 65535 ||
+      (int64_t)max_queries * G > 65535 * (int64_t)128)
+    return false;
+  p.max_keys = (int)keys;
+  p.pages_per_seq = (int)((keys + kFp4Page - 1) / kFp4Page);
+  const int64_t per_seq = (int64_t)p.pages_per_seq * kFp4Page * num_kv_heads * head_dim * 2;
+  const int64_t fit = kPageBytesMost / (2 * per_seq);
+  p.part = (int)(fit < 1 ? 1 : fit < batch ? fit : batch);
+  if ((int64_t)p.part * p.pages_per_seq > INT32_MAX) return false;
+  const auto pad = [](size_t x) { return (x + 255) / 256 * 256; };
+  p.cu_bytes = pad((size_t)2 * (batch + 1) * sizeof(int32_t));
+  p.table_bytes = pad((size_t)p.part * p.pages_per_seq * sizeof(int32_t));
+  p.page_bytes = (size_t)p.part * per_seq;
+  p.attn_bytes = pad(nvk_varlen_prefill_parts_workspace_size(p.part, max_queries, p.max_keys,
+                                                             num_q_heads, num_kv_heads, head_dim));
+  // the last part of the batch may be smaller, and cut its tiles into more parts
+  const int rest = batch % p.part;
+  if (rest) {
+    const size_t r = pad(nvk_varlen_prefill_parts_workspace_size(
+        rest, max_queries, p.max_keys, num_q_heads, num_kv_heads, head_dim));
+    p.attn_bytes = r > p.attn_bytes ? r : p.attn_bytes;
+  }
+  p.bytes = p.cu_bytes + p.table_bytes + 2 * p.page_bytes + p.attn_bytes;
+  return true;
+}
+
+int launch_pages(const AttnArgs& a, const PagePlan& p, int num_q_heads, float scale, bool f16,
+                 void* workspace, hipStream_t s) {
+  char* at = static_cast<char*>(workspace);
+  const int32_t *cu_q = a.cu_q, *cu_k = a.keys;
+  if (!cu_q) {
+    int32_t* cu = reinterpret_cast<int32_t*>(at);
+    const int st = nvk_uniform_cu_seqlens(a.keys, a.batch, a.n_query, cu, cu + a.batch + 1, s);
+    if (st != NVK_OK) return st;
+    cu_q = cu;
+    cu_k = cu + a.batch + 1;
+  }
+  at += p.cu_bytes;
+  Fp4Expand e{};
+  e.tables = reinterpret_cast<int32_t*>(at);
+  at += p.table_bytes;
+  e.k_pages = reinterpret_cast<uint16_t*>(at);
+  at += p.page_bytes;
+  e.v_pages = reinterpret_cast<uint16_t*>(at);
+  at += p.page_bytes;
+  e.k_data = a.k_data;
+  e.v_data = a.v_data;
+  e.k_scale = a.k_scale;
+  e.v_scale = a.v_scale;
+  e.bt_stride = a.bt_stride;
+  e.pages_per_seq = p.pages_per_seq;
+  e.max_blocks = a.cap / a.block_size;
+  e.block_size = a.block_size;
+  e.num_blocks = a.num_blocks;
+  e.num_kv_heads = a.num_kv_heads;
+  e.f16 = f16;
+  Fp4Prefill f{};
+  f.q = a.q;
+  f.q_stride_tok = a.q_stride_tok;
+  f.q_stride_head = a.q_stride_head;
+  f.total_q = a.total_q;
+  f.k_pages = e.k_pages;
+  f.v_pages = e.v_pages;
+  f.tables = e.tables;
+  f.max_seqlen_q = a.n_query;
+  f.max_seqlen_k = p.max_keys;
+  f.pages_per_seq = p.pages_per_seq;
+  f.num_q_heads = num_q_heads;
+  f.num_kv_heads = a.num_kv_heads;
+  f.scale = scale;
+  f.out = a.out;
+  f.out_stride_tok = a.out_stride_tok;
+  f.out_stride_head = a.out_stride_head;
+  f.workspace = at;
+  f.workspace_bytes = p.attn_bytes;
+  f.f16 = f16;
+  for (int b = 0; b < a.batch; b += p.part) {
+    e.batch = f.batch = a.batch - b < p.part ? a.batch - b : p.part;
+    e.block_tables = a.block_tables + b * a.bt_stride;
+    e.cu_k = f.cu_k = cu_k + b;
+    f.cu_q = cu_q + b;
+    int st = fp4_expand_launch(e, s);
+    if (st == NVK_OK) st = fp4_prefill_launch(f, s);
+    if (st != NVK_OK) return st;
+  }
+  return NVK_OK;
+}
+
 }  // namespace
 
 extern "C" size_t nvk_fp4_attention_workspace_size(int32_t batch, int32_t max_seqlen_q,
-                                                   int32_t num_q_heads, int32_t num_kv_heads,
-                                                   int32_t head_dim, int32_t block_size,
-                                                   int32_t max_blocks) {
+                                                   int32_t max_seqlen_k, int32_t num_q_heads,
+                                                   int32_t num_kv_heads, int32_t head_dim,
+                                                   int32_t block_size, int32_t max_blocks) {
   Plan p;
-  return plan_of(batch, max_seqlen_q, num_q_heads, num_kv_heads, head_dim, block_size, max_blocks, p)
-             ? p.bytes
-             : 0;
+  PagePlan pp;
+  if (!plan_of(batch, max_seqlen_q, num_q_heads, num_kv_heads, head_dim, block_size, max_blocks, p))
+    return 0;
+  return page_plan(batch, max_seqlen_q, max_seqlen_k, num_q_heads, num_kv_heads, head_dim,
+                   block_size, max_blocks, pp)
+             ? pp.bytes
+             : p.bytes;
 }
 
 extern "C" int nvk_fp4_attention(const void* q, int64_t q_stride_tok, int64_t q_stride_head,
                                  int64_t total_q, const void* k_data, const void* k_scale,
                                  const void* v_data, const void* v_scale,
                                  const int32_t* cu_seqlens_q, const int32_t* seqlens_k,
-                                 int32_t batch, int32_t max_seqlen_q, const int32_t* block_tables,
-                                 int64_t bt_stride, int32_t max_blocks, int32_t block_size,
-                                 int32_t num_blocks, int32_t num_q_heads, int32_t num_kv_heads,
-                                 int32_t head_dim, float scale, void* out, int64_t out_stride_tok,
+                                 int32_t batch, int32_t max_seqlen_q, int32_t max_seqlen_k,
+                                 const int32_t* block_tables, int64_t bt_stride,
+                                 int32_t max_blocks, int32_t block_size, int32_t num_blocks,
+                                 int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                                 float scale, void* out, int64_t out_stride_tok,
                                  int64_t out_stride_head, void* workspace, size_t workspace_bytes,
                                  int32_t dtype, void* stream) {
-  if (batch < 0 || total_q < 0 || max_seqlen_q < 0 || num_q_heads <= 0 || num_kv_heads <= 0 ||
+  if (batch < 0 || total_q < 0 || max_seqlen_q < 0 || max_seqlen_k < 0 || num_q_heads <= 0 || num_kv_heads <= 0 ||
       block_size <= 0 || max_blocks < 0 || num_blocks < 0 || num_q_heads % num_kv_heads)
     return NVK_EINVAL;
   if (!(scale > 0.f)) return NVK_EINVAL;
@@ -635,7 +749,10 @@ extern "C" int nvk_fp4_attention(const void* q, int64_t q_stride_tok, int64_t q_
   if ((uintptr_t)out % 8 || out_stride_tok % 4 || out_stride_head % 4) return NVK_EALIGN;
   if (((uintptr_t)cu_seqlens_q | (uintptr_t)seqlens_k | (uintptr_t)block_tables) % 4)
     return NVK_EALIGN;
-  if (!workspace || workspace_bytes < p.bytes) return NVK_EWORKSPACE;
+  PagePlan pp;
+  const bool pages = page_plan(batch, max_seqlen_q, max_seqlen_k, num_q_heads, num_kv_heads,
+                               head_dim, block_size, max_blocks, pp);
+  if (!workspace || workspace_bytes < (pages ? pp.bytes : p.bytes)) return NVK_EWORKSPACE;
   if ((uintptr_t)workspace % 256) return NVK_EALIGN;
   AttnArgs a{};
   a.q = static_cast<const uint16_t*>(q);
@@ -668,6 +785,7 @@ extern "C" int nvk_fp4_attention(const void* q, int64_t q_stride_tok, int64_t q_
   a.n_waves = p.n_waves;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const bool f16 = dtype == NVK_DTYPE_F16;
+  if (pages) return launch_pages(a, pp, num_q_heads, scale, f16, workspace, s);
   if (head_dim == 128) return f16 ? launch<128, true>(a, s) : launch<128, false>(a, s);
   return f16 ? launch<64, true>(a, s) : launch<64, false>(a, s);
 }

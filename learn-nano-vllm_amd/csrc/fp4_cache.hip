@@ -142,6 +142,78 @@ __global__ __launch_bounds__(256) void fp4_load_kernel(CacheArgs a, uint16_t* ke
   *reinterpret_cast<nvk_u32x4*>(value + t * value_stride + col) = v;
 }
 
+// Keys and values of each sequence's pages as f16 (see Fp4Expand).  grid = (64-token pieces of a
+// sequence, kv heads, sequences); 16 lanes a row, 16 rows a pass.
+template <bool F16>
+__global__ __launch_bounds__(256) void fp4_expand_kernel(Fp4Expand a) {
+  constexpr int HD = 128, kPass = 4;
+  const int s = blockIdx.z, h = blockIdx.y;
+  if (blockIdx.x == 0 && h == 0)
+    for (int i = threadIdx.x; i < a.pages_per_seq; i += 256)
+      a.tables[(int64_t)s * a.pages_per_seq + i] = s * a.pages_per_seq + i;
+  int64_t keys = (int64_t)a.cu_k[s + 1] - a.cu_k[s];
+  if (keys > (int64_t)a.pages_per_seq * kFp4Page) keys = (int64_t)a.pages_per_seq * kFp4Page;
+  if (keys > (int64_t)a.max_blocks * a.block_size) keys = (int64_t)a.max_blocks * a.block_size;
+  const int u = threadIdx.x % 16;
+  const int p0 = blockIdx.x * 16 * kPass + threadIdx.x / 16;
+  const int32_t* bt = a.block_tables + s * a.bt_stride;
+  uint32_t kc[kPass], vc[kPass];
+  uint16_t ks[kPass], vs[kPass];
+#pragma unroll
+  for (int i = 0; i < kPass; ++i) {
+    const int p = p0 + 16 * i;
+    if (p >= keys) continue;
+    const int logical = p / a.block_size;
+    int page = bt[logical];
+    if (page < 0 || page >= a.num_blocks) page = 0;
+    const int off = p - logical * a.block_size;
+    const int64_t head = (int64_t)page * a.num_kv_heads + h;
+    const int64_t row = head * a.block_size + off;
+    const int64_t srow = head * 4 * a.block_size + off + (int64_t)(u / 4) * a.block_size;
+    kc[i] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(
+        a.k_data + row * (HD / 2) + 4 * fp4_place<HD, true>(u)));
+    vc[i] = __builtin_nontemporal_load(
+        reinterpret_cast<const uint32_t*>(a.v_data + row * (HD / 2) + 4 * u));
+    ks[i] = a.k_scale[srow];
+    vs[i] = a.v_scale[srow];
+  }
+  auto f16_values = [](uint32_t code, float s) {
+    const auto c = __builtin_bit_cast(nvk_u32x4, fp4_unpack<true>(code));
+    nvk_u32x4 o;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float lo = NvkElt<true>::lo(c[i]) * s, hi = NvkElt<true>::hi(c[i]) * s;
+      if constexpr (F16) {  // fmin / fmax drop a NaN: it goes into the keys below
+        lo = fminf(fmaxf(lo, -65504.f), 65504.f);
+        hi = fminf(fmaxf(hi, -65504.f), 65504.f);
+      }
+      o[i] = NvkElt<true>::pack2(lo, hi);
+    }
+    return o;
+  };
+  constexpr float kUnit = F16 ? 1.f : 1.f / (1 << kFp4KeyShift);
+#pragma unroll
+  for (int i = 0; i < kPass; ++i) {
+    const int p = p0 + 16 * i;
+    if (p >= keys) continue;  // whole rows: the lanes of a row leave together
+    const float fk = (float)__builtin_bit_cast(_Float16, ks[i]) * kUnit;
+    float fv = (float)__builtin_bit_cast(_Float16, vs[i]) * kUnit;
+    // A value that is not finite would meet the zero probability of a query that does not see
+    // it, as NaN.  It becomes 0 here and the row's key NaN, whose score a mask replaces.
+    const bool lost = !__builtin_isfinite(fk) || !__builtin_isfinite(fv);
+    const bool row_lost =
+        (__builtin_amdgcn_ballot_w64(lost) >> (threadIdx.x & 48) & 0xffffu) != 0;
+    if (!__builtin_isfinite(fv)) fv = 0.f;
+    nvk_u32x4 k = f16_values(kc[i], fk);
+    const nvk_u32x4 v = f16_values(vc[i], fv);
+    if (row_lost) k = nvk_u32x4{0x7e007e00u, 0x7e007e00u, 0x7e007e00u, 0x7e007e00u};
+    const int64_t at =
+        (((int64_t)s * a.pages_per_seq * kFp4Page + p) * a.num_kv_heads + h) * HD + 8 * u;
+    *reinterpret_cast<nvk_u32x4*>(a.k_pages + at) = k;
+    *reinterpret_cast<nvk_u32x4*>(a.v_pages + at) = v;
+  }
+}
+
 // The checks that store and load share; fills `a`.
 int cache_args(CacheArgs& a, const void* rows_k, int64_t key_row_stride, const void* rows_v,
                int64_t value_row_stride, void* k_data, void* k_scale, void* v_data, void* v_scale,
@@ -213,6 +285,15 @@ struct LoadLaunch {
 };
 
 }  // namespace
+
+int fp4_expand_launch(const Fp4Expand& p, hipStream_t stream) {
+  const dim3 grid(p.pages_per_seq * (kFp4Page / 64), p.num_kv_heads, p.batch);
+  if (p.f16)
+    hipLaunchKernelGGL(fp4_expand_kernel<true>, grid, dim3(256), 0, stream, p);
+  else
+    hipLaunchKernelGGL(fp4_expand_kernel<false>, grid, dim3(256), 0, stream, p);
+  return nvk_launch_status();
+}
 
 extern "C" int nvk_fp4_store(const void* key, int64_t key_row_stride, const void* value,
                              int64_t value_row_stride, void* k_data, void* k_scale, void* v_data,

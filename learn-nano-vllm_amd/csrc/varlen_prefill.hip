@@ -47,6 +47,7 @@
 
 #include "nvk_common.h"
 #include "qk_math.h"
+#include "fp4.h"
 #include "qk_prologue.h"
 #include "short_query.h"
 
@@ -110,6 +111,9 @@ struct PrefillArgs {
   float eps;
   const float* cos_sin;
   int64_t cos_sin_stride, max_position;
+  // q and out are bf16, k and v f16 times 2^-kFp4KeyShift (pages expanded from a
+  // 4-bit cache).
+  bool mixed;
 };
 
 // Partial record of one (query tile, part): the unnormalised O^T accumulators
@@ -326,10 +330,18 @@ __device__ __forceinline__ void wait_lds_loads() {
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
-template <int G, int MODE, bool F16, bool QN>
+// MIXED (with F16): q and out are bf16, see PrefillArgs::mixed.  q becomes f16, which
+// bf16's 8 bits fit but not its range: a wave whose largest |q| is outside [2^-6, 2^15)
+// takes its rows times a power of two, and the scores' scale the inverse.  f16
+// keys, values and probabilities are off by 2^-11 at most where bf16 ones are off by 2^-8:
+// against 64 bits, a chunk of 1000 after 8300 and 32 x U{100..1024} after 512 are 0.0017
+// off, 0.0029 with all of them in bf16 (the output's own rounding: 0.0017), at the same time.
+template <int G, int MODE, bool F16, bool QN, bool MIXED = false>
 __global__ __launch_bounds__(64 * kWaves, 8 / kWaves) void varlen_prefill_kernel(PrefillArgs a) {
+  static_assert(!MIXED || (F16 && !QN), "bf16 rows over f16 keys");
   constexpr int TQ = kRows / G;  // query tokens per workgroup
   using E = NvkElt<F16>;
+  using EO = NvkElt<F16 && !MIXED>;  // of the output
   typedef typename E::vec8 vec8;
 
   const int kvh = blockIdx.x;
@@ -380,6 +392,7 @@ __global__ __launch_bounds__(64 * kWaves, 8 / kWaves) void varlen_prefill_kernel
   const int head = kvh * G + row % G;
   const bool row_valid = tok >= 0 && tok < Lq;
   vec8 qf[HD / 16];
+  float scale_log2 = a.scale_log2;
   // QN: the raw rows, the norm weights and the cos / sin, loaded here and
   // applied once the first key tiles are under way
   nvk_u32x4 q_raw[HD / 16], q_w[HD / 16], q_cs[4][4];
@@ -415,6 +428,40 @@ __global__ __launch_bounds__(64 * kWaves, 8 / kWaves) void varlen_prefill_kernel
         qf[ks] = __builtin_bit_cast(vec8, w);
       }
     }
+  }
+  if constexpr (MIXED) {
+    uint32_t top = 0;  // the largest |q| of the wave, as bf16 bits
+#pragma unroll
+    for (int ks = 0; ks < HD / 16; ++ks) {
+      const nvk_u32x4 w = __builtin_bit_cast(nvk_u32x4, qf[ks]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t lo = w[i] & 0x7fffu, hi = w[i] >> 16 & 0x7fffu;
+        top = top > lo ? top : lo;
+        top = top > hi ? top : hi;
+      }
+    }
+    float t = __uint_as_float(top << 16);
+    t = fmaxf(t, nvk_dpp<NVK_DPP_QP_XOR1>(t));
+    t = fmaxf(t, nvk_dpp<NVK_DPP_QP_XOR2>(t));
+    t = fmaxf(t, nvk_dpp<NVK_DPP_HALF_MIRROR>(t));
+    t = fmaxf(t, nvk_dpp<NVK_DPP_MIRROR>(t));
+    t = fmaxf(t, nvk_xor_lane<16>(t));
+    t = nvk_max_xor32(t);
+    const int e = (int)(__float_as_uint(t) >> 23);  // biased exponent; 0: all zero (or subnormal)
+    int shift = e >= 127 - 6 && e < 127 + 15 ? 0 : e - 127;
+    shift = __builtin_amdgcn_readfirstlane(e == 255 || e == 0 ? 0 : shift);
+#pragma unroll
+    for (int ks = 0; ks < HD / 16; ++ks) {
+      nvk_u32x4 w = __builtin_bit_cast(nvk_u32x4, qf[ks]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        w[i] = E::pack2(__builtin_ldexpf(EO::lo(w[i]), -shift),
+                        __builtin_ldexpf(EO::hi(w[i]), -shift));
+      qf[ks] = __builtin_bit_cast(vec8, w);
+    }
+    scale_log2 = __uint_as_float((uint32_t)__builtin_amdgcn_readfirstlane(
+        (int)__float_as_uint(__builtin_ldexpf(a.scale_log2, shift + kFp4KeyShift))));
   }
   const int row_limit = tok + diag;  // last visible key of this row
 
@@ -665,7 +712,7 @@ __global__ __launch_bounds__(64 * kWaves, 8 / kWaves) void varlen_prefill_kernel
   };
   auto max_join_b = [&](const nvk_f32x16 (&sc)[2], const float (&t)[2]) -> float {
     const float u = nvk_max3(t[0], t[1], sc[1][7]);
-    return nvk_max_xor32(fmaxf(u, sc[1][15])) * a.scale_log2;  // tile max, log2 units
+    return nvk_max_xor32(fmaxf(u, sc[1][15])) * scale_log2;  // tile max, log2 units
   };
   // Lazy rescale for a tile whose row max (log2 units) is mt; returns the
   // offset for exp2.
@@ -698,8 +745,8 @@ __global__ __launch_bounds__(64 * kWaves, 8 / kWaves) void varlen_prefill_kernel
     const int p = n >> 2, e = n & 3;
     const int mb = p >> 1, i = 8 * (p & 1) + 2 * e;
     ExpPair x;
-    x.p0 = nvk_fast_exp2(fmaf(sc[mb][i], a.scale_log2, -moff));
-    x.p1 = nvk_fast_exp2(fmaf(sc[mb][i + 1], a.scale_log2, -moff));
+    x.p0 = nvk_fast_exp2(fmaf(sc[mb][i], scale_log2, -moff));
+    x.p1 = nvk_fast_exp2(fmaf(sc[mb][i + 1], scale_log2, -moff));
     asm volatile("" : "+v"(x.p0), "+v"(x.p1));  // issued here
     return x;
   };
@@ -1002,12 +1049,12 @@ __global__ __launch_bounds__(64 * kWaves, 8 / kWaves) void varlen_prefill_kernel
     }
     return;
   }
-  const float inv = l_tot > 0.f ? 1.f / l_tot : 0.f;
+  const float inv = (l_tot > 0.f ? 1.f / l_tot : 0.f) * (MIXED ? (float)(1 << kFp4KeyShift) : 1.f);
   // Lane (half, l32) holds d = 32 db + 8 grp + 4 half .. +3 of its row.
   auto packed = [&](int db, int grp) {
     nvk_u32x2 w;
-    w.x = E::pack2(acc_o[db][4 * grp] * inv, acc_o[db][4 * grp + 1] * inv);
-    w.y = E::pack2(acc_o[db][4 * grp + 2] * inv, acc_o[db][4 * grp + 3] * inv);
+    w.x = EO::pack2(acc_o[db][4 * grp] * inv, acc_o[db][4 * grp + 1] * inv);
+    w.y = EO::pack2(acc_o[db][4 * grp + 2] * inv, acc_o[db][4 * grp + 3] * inv);
     return w;
   };
   if (!a.out_rows16) {  // 8 bytes per lane and store (16 per row and instruction)
@@ -1062,10 +1109,10 @@ __global__ __launch_bounds__(64 * kWaves, 8 / kWaves) void varlen_prefill_kernel
 // loads in flight.  The normalised rows go through LDS so that each store
 // writes whole 256-byte rows.
 constexpr int kFoldBatch = 4;
-template <int G, int MODE, bool F16>
+template <int G, int MODE, bool F16, bool MIXED = false>
 __global__ __launch_bounds__(256) void prefill_combine_kernel(PrefillArgs a) {
   constexpr int TQ = kRows / G;
-  using E = NvkElt<F16>;
+  using E = NvkElt<F16 && !MIXED>;
   const int kvh = blockIdx.x / kWaves, w = blockIdx.x % kWaves, s = blockIdx.y, qt = blockIdx.z;
   const QTile qi = qtile_info<MODE>(a, s, qt, TQ);
   if (!qi.live) return;
@@ -1116,7 +1163,7 @@ __global__ __launch_bounds__(256) void prefill_combine_kernel(PrefillArgs a) {
       for (int i = 0; i < 4; ++i) acc[i] += wt * ov[v][i];
     }
   }
-  const float inv = L > 0.f ? 1.f / L : 0.f;
+  const float inv = (L > 0.f ? 1.f / L : 0.f) * (MIXED ? (float)(1 << kFp4KeyShift) : 1.f);
   // quad 4u + i of a lane: d = 32 u + 8 i + 4 half .. +3 of its row
   __shared__ __attribute__((aligned(16))) uint8_t rows[32 * HD * 2];
 #pragma unroll
@@ -1146,10 +1193,13 @@ __global__ __launch_bounds__(256) void prefill_combine_kernel(PrefillArgs a) {
   }
 }
 
-template <int G, int MODE, bool F16>
+template <int G, int MODE, bool F16, bool MIXED = false>
 int launch_mode(const PrefillArgs& a, hipStream_t stream) {
   dim3 grid(a.num_kv_heads, a.batch, a.n_qtiles * a.n_splits);
-  if (a.positions)
+  if constexpr (MIXED)
+    hipLaunchKernelGGL((varlen_prefill_kernel<G, MODE, F16, false, true>), grid,
+                       dim3(64 * kWaves), 0, stream, a);
+  else if (a.positions)
     hipLaunchKernelGGL((varlen_prefill_kernel<G, MODE, F16, true>), grid, dim3(64 * kWaves), 0,
                        stream, a);
   else
@@ -1159,13 +1209,15 @@ int launch_mode(const PrefillArgs& a, hipStream_t stream) {
     const int st = nvk_launch_status();
     if (st != NVK_OK) return st;
     dim3 cgrid(a.num_kv_heads * kWaves, a.batch, a.n_qtiles);
-    hipLaunchKernelGGL((prefill_combine_kernel<G, MODE, F16>), cgrid, dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((prefill_combine_kernel<G, MODE, F16, MIXED>), cgrid, dim3(256), 0, stream, a);
   }
   return nvk_launch_status();
 }
 
 template <int G, bool F16>
 int launch_prefill(const PrefillArgs& a, hipStream_t stream) {
+  if constexpr (F16)
+    if (a.mixed) return launch_mode<G, kPagedAligned, true, true>(a, stream);
   if (!a.block_tables) return launch_mode<G, kDense, F16>(a, stream);
   // aligned pages whose byte size fits 32 bits (tile addresses in 32 x 32-bit products)
   if (a.block_size % kKeys == 0 &&
@@ -1375,7 +1427,8 @@ int varlen_prefill_impl(const void* q, int64_t q_stride_tok, int64_t q_stride_he
                         int32_t head_dim, float scale, void* out, int64_t out_stride_tok,
                         int64_t out_stride_head, void* workspace, size_t workspace_bytes,
                         int32_t dtype, void* stream, const int32_t* given_order,
-                        size_t given_order_bytes, const QkPrologue* pro = nullptr) {
+                        size_t given_order_bytes, const QkPrologue* pro = nullptr,
+                        bool mixed = false) {
   if (batch < 0 || max_seqlen_q < 0 || max_seqlen_k < 0 || num_q_heads <= 0 ||
       num_kv_heads <= 0 || total_q < 0 || total_k < 0)
     return NVK_EINVAL;
@@ -1510,6 +1563,7 @@ int varlen_prefill_impl(const void* q, int64_t q_stride_tok, int64_t q_stride_he
   a.n_splits = sp.n_splits;
   a.tiles_per_split = sp.n_splits > 1 ? sp.tiles_per_split : 1 << 30;
   a.ws = static_cast<float*>(workspace);
+  a.mixed = mixed;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   // One query tile per workgroup, a grid of several rounds and room in the
   // workspace: rank the tiles longest first (one more small kernel).  One
@@ -1538,6 +1592,16 @@ int varlen_prefill_impl(const void* q, int64_t q_stride_tok, int64_t q_stride_he
 }
 
 }  // namespace
+
+int fp4_prefill_launch(const Fp4Prefill& p, hipStream_t stream) {
+  return varlen_prefill_impl(
+      p.q, p.q_stride_tok, p.q_stride_head, p.total_q, p.k_pages, p.v_pages, 0, 0, 0,
+      (int64_t)p.batch * p.pages_per_seq * kFp4Page, p.cu_q, p.cu_k, p.batch, p.max_seqlen_q,
+      p.max_seqlen_k, p.tables, p.pages_per_seq, p.pages_per_seq, kFp4Page,
+      p.batch * p.pages_per_seq, p.num_q_heads, p.num_kv_heads, HD, p.scale, p.out,
+      p.out_stride_tok, p.out_stride_head, p.workspace, p.workspace_bytes, NVK_DTYPE_F16, stream,
+      nullptr, 0, nullptr, !p.f16);
+}
 
 extern "C" int nvk_varlen_prefill(const void* q, int64_t q_stride_tok, int64_t q_stride_head,
                                   int64_t total_q, const void* k, const void* v,

@@ -106,10 +106,10 @@ SIGNATURES = {
                                     _c_i32, _c_i32, _c_ptr, _c_i64, _c_ptr, _c_i64, _c_i32,
                                     _c_ptr]),
     "nvk_fp4_attention_workspace_size": (ctypes.c_size_t, [_c_i32, _c_i32, _c_i32, _c_i32, _c_i32,
-                                                           _c_i32, _c_i32]),
+                                                           _c_i32, _c_i32, _c_i32]),
     "nvk_fp4_attention": (ctypes.c_int, [_c_ptr, _c_i64, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_ptr,
-                                         _c_ptr, _c_ptr, _c_ptr, _c_i32, _c_i32, _c_ptr, _c_i64,
-                                         _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32,
+                                         _c_ptr, _c_ptr, _c_ptr, _c_i32, _c_i32, _c_i32, _c_ptr,
+                                         _c_i64, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32,
                                          ctypes.c_float, _c_ptr, _c_i64, _c_i64, _c_ptr,
                                          ctypes.c_size_t, _c_i32, _c_ptr]),
     "nvk_gather_last_tokens": (ctypes.c_int, [_c_ptr, _c_i64, _c_ptr, _c_i32, _c_i32, _c_i32, _c_ptr,

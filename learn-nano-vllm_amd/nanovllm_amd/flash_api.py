@@ -85,7 +85,8 @@ def varlen_prefill(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, softmax_sc
         if block_table is None:
             raise _lib.NvkError("a 4-bit cache is read through a block_table")
         return fp4_attention(q, k, v, cu_seqlens_k, block_table, softmax_scale,
-                             cu_seqlens_q=cu_seqlens_q, max_seqlen_q=max_seqlen_q, out=out)
+                             cu_seqlens_q=cu_seqlens_q, max_seqlen_q=max_seqlen_q,
+                             max_seqlen_k=max_seqlen_k, out=out)
     dev = _lib.require_gpu(q, k, v, cu_seqlens_q, cu_seqlens_k, block_table)
     dtype = _attn_dtype(q, k, v)
     if q.dim() != 3 or q.stride(-1) != 1:

@@ -121,11 +121,12 @@ def load_kvcache(k_cache: Fp4Cache, v_cache: Fp4Cache, slot_mapping: torch.Tenso
 
 def fp4_attention(q: torch.Tensor, k_cache: Fp4Cache, v_cache: Fp4Cache, seqlens_k: torch.Tensor,
                   block_table: torch.Tensor, softmax_scale=None, cu_seqlens_q=None,
-                  max_seqlen_q: int = 1, out: torch.Tensor | None = None) -> torch.Tensor:
+                  max_seqlen_q: int = 1, max_seqlen_k: int | None = None,
+                  out: torch.Tensor | None = None) -> torch.Tensor:
     """Causal attention of q [tokens, Hq, D] over 4-bit caches.  Without ``cu_seqlens_q`` every
     sequence has ``max_seqlen_q`` queries and ``seqlens_k`` [B] keys; with it both are prefix sums
-    [B + 1].  The queries are the last of their sequence's keys.  Returns [tokens, Hq, D] (or fills
-    ``out``)."""
+    [B + 1].  The queries are the last of their sequence's keys.  ``max_seqlen_k`` bounds the keys of
+    a sequence (None: what the block table holds).  Returns [tokens, Hq, D] (or fills ``out``)."""
     nb, bs, hkv, d = _check_caches(k_cache, v_cache)
     dev = _lib.require_gpu(q, *k_cache, *v_cache, seqlens_k, block_table, cu_seqlens_q)
     dtype = _rows_dtype(q.dtype)
@@ -148,15 +149,15 @@ def fp4_attention(q: torch.Tensor, k_cache: Fp4Cache, v_cache: Fp4Cache, seqlens
         raise _lib.NvkError("out must be like q, with unit last stride")
     scale = float(softmax_scale) if softmax_scale is not None else d ** -0.5
     lib = _lib.load()
-    mq, width = int(max_seqlen_q), bt.shape[1]
-    ws_bytes = lib.nvk_fp4_attention_workspace_size(batch, mq, hq, hkv, d, bs, width)
+    mq, mk, width = int(max_seqlen_q), int(max_seqlen_k or 0), bt.shape[1]
+    ws_bytes = lib.nvk_fp4_attention_workspace_size(batch, mq, mk, hq, hkv, d, bs, width)
     ws = _lib.workspace(dev, ws_bytes)
     with _lib.on_device(dev):
         code = lib.nvk_fp4_attention(
             q.data_ptr(), q.stride(0), q.stride(1), tq, k_cache.data.data_ptr(),
             k_cache.scale.data_ptr(), v_cache.data.data_ptr(), v_cache.scale.data_ptr(),
-            _lib.ptr(cu_q), lens.data_ptr(), batch, mq, bt.data_ptr(), bt.stride(0), width, bs, nb,
-            hq, hkv, d, scale, out.data_ptr(), out.stride(0), out.stride(1), _lib.ptr(ws),
+            _lib.ptr(cu_q), lens.data_ptr(), batch, mq, mk, bt.data_ptr(), bt.stride(0), width, bs,
+            nb, hq, hkv, d, scale, out.data_ptr(), out.stride(0), out.stride(1), _lib.ptr(ws),
             ws_bytes, dtype, _lib.stream_ptr(dev))
     _lib.check(code)
     return out

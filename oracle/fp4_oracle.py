@@ -73,14 +73,22 @@ def store(rows, data, scale, slots, keys):
             scale[slot // p, :, :, slot % p] = s[t]
 
 
-def attention(q, k, v, n_keys, scale):
+def through_pages(n, g, d):
+    """Whether n queries of g heads per kv head run over f16 pages of the keys and values."""
+    return n * g > 128 and d == 128 and g in (1, 2, 4, 8)
+
+
+def attention(q, k, v, n_keys, scale, pages=False):
     """One sequence: q [n, Hq, D], k / v [>= n_keys, Hkv, D]; query i sees keys j <= i + n_keys - n.
     Returns (out, size) [n, Hq, D]: the attention, and what its rounding errors are relative to:
     `size` bounds |kernel - out| without the rounding of the output itself.
 
     The kernel's probabilities are off by a relative 2 (D + 8) 2^-24 sum |q_i k_i| scale (the f32 sum of
     the score, in e^x, against the maximum) and, times the value's scale, by half a step of f16
-    (2^-11 relative, 2^-25 at least); n_keys f32 additions and the exponential add 2 (n + 64) 2^-24."""
+    (2^-11 relative, 2^-25 at least); n_keys f32 additions and the exponential add 2 (n + 64) 2^-24.
+    pages: keys, values and probabilities are off by half a step of f16 each, keys and values by 2^-22
+    at least (f16 holds an eighth of them): in a score, that is 2^-11 sum |q_i k_i| scale
+    + 2^-22 sum |q_i| scale, twice (against the maximum)."""
     n, hq, d = q.shape
     g = hq // k.shape[1]
     out, size = np.zeros((n, hq, d)), np.zeros((n, hq, d))
@@ -96,5 +104,8 @@ def attention(q, k, v, n_keys, scale):
             l = e.sum()
             out[i, h] = e @ vv[:m] / l
             rel = 2 * (d + 8) * 2.0 ** -24 * off + 2.0 ** -11 + 2 * (m + 64) * 2.0 ** -24
+            if pages:
+                rel += 2.0 ** -11 * (1 + 2 * off) + 2.0 ** -21 * np.abs(q[i, h]).sum() * scale
             size[i, h] = rel * (e @ np.abs(vv[:m]) / l) + 2.0 ** -25 * 6 * m / l
+            size[i, h] += 2.0 ** -22 if pages else 0.0
     return out, size

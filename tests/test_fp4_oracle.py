@@ -132,30 +132,36 @@ def test_error_codes_without_launching():
     assert lib.nvk_fp4_load(*change(ld, a10=None)) == EINVAL
     assert lib.nvk_fp4_load(*change(ld, a14=2)) == EUNSUPPORTED
     assert lib.nvk_fp4_load(*change(ld, a12=8)) == EALIGN
-    # q, strides, total_q, caches, cu_q, seqlens, batch, max_q, table, stride, width, bs, nb, hq,
-    # hkv, d, scale, out, strides, workspace, bytes, dtype, stream
-    need = lib.nvk_fp4_attention_workspace_size(2, 1, 16, 8, 128, 256, 8)
+    # q, strides, total_q, caches, cu_q, seqlens, batch, max_q, max_k, table, stride, width, bs,
+    # nb, hq, hkv, d, scale, out, strides, workspace, bytes, dtype, stream
+    need = lib.nvk_fp4_attention_workspace_size(2, 1, 0, 16, 8, 128, 256, 8)
     assert need > 0
-    at = [16, 2048, 128, 2, 16, 16, 16, 16, None, 16, 2, 1, 16, 8, 8, 256, 64, 16, 8, 128, 0.1, 16,
+    at = [16, 2048, 128, 2, 16, 16, 16, 16, None, 16, 2, 1, 0, 16, 8, 8, 256, 64, 16, 8, 128, 0.1, 16,
           2048, 128, 256, need, 0, None]
     assert lib.nvk_fp4_attention(*change(at, a3=0, a10=0)) == 0
     assert lib.nvk_fp4_attention(*change(at, a3=3)) == EINVAL         # 2 sequences, 3 queries
-    assert lib.nvk_fp4_attention(*change(at, a20=0.0)) == EINVAL
-    assert lib.nvk_fp4_attention(*change(at, a17=12)) == EINVAL       # 12 % 8
-    assert lib.nvk_fp4_attention(*change(at, a13=4)) == EINVAL        # tables overlap
+    assert lib.nvk_fp4_attention(*change(at, a21=0.0)) == EINVAL
+    assert lib.nvk_fp4_attention(*change(at, a12=-1)) == EINVAL
+    assert lib.nvk_fp4_attention(*change(at, a18=12)) == EINVAL       # 12 % 8
+    assert lib.nvk_fp4_attention(*change(at, a14=4)) == EINVAL        # tables overlap
     assert lib.nvk_fp4_attention(*change(at, a9=None)) == EINVAL
-    assert lib.nvk_fp4_attention(*change(at, a19=96)) == EUNSUPPORTED
-    assert lib.nvk_fp4_attention(*change(at, a15=8)) == EUNSUPPORTED
-    assert lib.nvk_fp4_attention(*change(at, a16=0)) == EUNSUPPORTED  # no page
-    assert lib.nvk_fp4_attention(*change(at, a17=256)) == EUNSUPPORTED  # 32 heads per kv head
-    assert lib.nvk_fp4_attention(*change(at, a26=2)) == EUNSUPPORTED
+    assert lib.nvk_fp4_attention(*change(at, a20=96)) == EUNSUPPORTED
+    assert lib.nvk_fp4_attention(*change(at, a16=8)) == EUNSUPPORTED
+    assert lib.nvk_fp4_attention(*change(at, a17=0)) == EUNSUPPORTED  # no page
+    assert lib.nvk_fp4_attention(*change(at, a18=256)) == EUNSUPPORTED  # 32 heads per kv head
+    assert lib.nvk_fp4_attention(*change(at, a27=2)) == EUNSUPPORTED
     assert lib.nvk_fp4_attention(*change(at, a0=8)) == EALIGN
     assert lib.nvk_fp4_attention(*change(at, a2=132)) == EALIGN
-    assert lib.nvk_fp4_attention(*change(at, a21=20)) == EALIGN
-    assert lib.nvk_fp4_attention(*change(at, a24=None)) == EWORKSPACE
-    assert lib.nvk_fp4_attention(*change(at, a25=need - 1)) == EWORKSPACE
-    assert lib.nvk_fp4_attention(*change(at, a24=128)) == EALIGN
+    assert lib.nvk_fp4_attention(*change(at, a22=20)) == EALIGN
+    assert lib.nvk_fp4_attention(*change(at, a25=None)) == EWORKSPACE
+    assert lib.nvk_fp4_attention(*change(at, a26=need - 1)) == EWORKSPACE
+    assert lib.nvk_fp4_attention(*change(at, a25=128)) == EALIGN
     size = lib.nvk_fp4_attention_workspace_size
-    assert size(2049, 1, 16, 8, 128, 256, 8) == 0 and size(2, 1, 16, 8, 128, 24, 8) == 0
-    assert size(2, 0, 16, 8, 128, 256, 8) == 0 and size(2, 1, 16, 5, 128, 256, 8) == 0
-    assert size(2048, 4096, 16, 1, 128, 256, 1 << 20) == 0            # past 32-bit work counts
+    assert size(2049, 1, 0, 16, 8, 128, 256, 8) == 0 and size(2, 1, 0, 16, 8, 128, 24, 8) == 0
+    assert size(2, 0, 0, 16, 8, 128, 256, 8) == 0 and size(2, 1, 0, 16, 5, 128, 256, 8) == 0
+    assert size(2048, 4096, 0, 16, 1, 128, 256, 1 << 20) == 0         # past 32-bit work counts
+    # many queries: f16 pages of the keys, 512 MiB of them or one sequence's, and no more with a
+    # bound on the keys
+    assert size(1, 1000, 9300, 16, 8, 128, 256, 64) > 2 * 37 * 256 * 8 * 128 * 2
+    assert size(1, 1000, 9300, 16, 8, 128, 256, 64) < size(1, 1000, 0, 16, 8, 128, 256, 64)
+    assert size(64, 1000, 9300, 16, 8, 128, 256, 64) < 700 << 20

@@ -13,14 +13,16 @@ from oracle import fp4_oracle as orc
 pytestmark = pytest.mark.gpu
 
 
-def _reference(q, pages, tables, n_queries, lens, scale):
-    """Oracle of sequences whose queries follow each other in q [tokens, Hq, D]."""
+def _reference(q, pages, tables, n_queries, lens, scale, longest=None):
+    """Oracle of sequences whose queries follow each other in q [tokens, Hq, D]; longest: the most
+    queries that the call was told of."""
     qn = q.double().cpu().numpy()
+    through = orc.through_pages(longest or max(n_queries), q.shape[1] // pages.hkv, pages.d)
     out, size = np.zeros(qn.shape), np.zeros(qn.shape)
     at = 0
     for b, (n, m) in enumerate(zip(n_queries, lens)):
         k, v = pages.rows(tables[b], m)
-        out[at:at + n], size[at:at + n] = orc.attention(qn[at:at + n], k, v, m, scale)
+        out[at:at + n], size[at:at + n] = orc.attention(qn[at:at + n], k, v, m, scale, through)
         at += n
     return out, size
 
@@ -61,7 +63,7 @@ def test_decode_of_contexts_cut_into_many_parts(lens, bs):
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
 @pytest.mark.parametrize("n,hq,hkv,d", [(2, 16, 8, 128), (6, 16, 8, 128), (8, 16, 8, 128),
-                                        (5, 8, 1, 128), (33, 4, 2, 128), (3, 4, 4, 64),
+                                        (5, 8, 1, 128), (33, 4, 2, 128), (70, 4, 2, 128), (3, 4, 4, 64),
                                         (70, 2, 2, 64)])
 def test_several_queries_of_every_sequence(n, hq, hkv, d, dtype):
     lens = [n, n + 1, 64, 300, 130, max(0, n - 1), 0]     # two with rows that see no key
@@ -99,6 +101,94 @@ def test_ragged_queries(news, cached, bs, dtype):
     got = flash_attn_varlen_func(q, *pages.gpu(), cu(news), cu(lens), max(news), max(lens),
                                  causal=True, block_table=_int(tables))
     assert torch.equal(got[:total], out[:total])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("hq,hkv,bs", [(2, 2, 256), (4, 2, 16), (4, 1, 64), (8, 1, 48), (3, 1, 64)])
+def test_chunks_of_many_queries(hq, hkv, bs, dtype):
+    """Over f16 pages (three heads per kv head: without), with chunks that end inside a tile, in front
+    of everything, and sequences without queries or with fewer keys than queries."""
+    news, cached = [150, 33, 0, 64, 40], [300, 0, 20, 65, -10]
+    lens = [a + b for a, b in zip(news, cached)]
+    tables, nb = tables_of(lens, bs, 8)
+    pages = Pages(12, nb, bs, hkv, 128, dtype)
+    q = rng_rows(13, (sum(news), hq, 128), dtype).cuda()
+    cu = lambda v: _int(np.concatenate([[0], np.cumsum(v)]))
+    say(f"fp4 chunks {hq}/{hkv} pages {bs} {dtype}")
+    for mk in (None, max(lens)):
+        out = varlen_prefill(q, *pages.gpu(), cu(news), cu(lens), max(news), None,
+                             block_table=_int(tables), max_seqlen_k=mk)
+        ref, size = _reference(q, pages, tables, news, lens, 128 ** -0.5)
+        assert_close(out, ref, size, dtype, "fp4 chunks")
+
+
+@pytest.mark.parametrize("up", [2.0 ** 20, 2.0 ** -20])
+def test_chunks_of_queries_far_from_one(up):
+    """bf16 queries outside f16's range, and values that only an eighth of fits it."""
+    hq, hkv, n = 2, 1, 70
+    tables, nb = tables_of([90], 64, 8)
+    pages = Pages(12, nb, 64, hkv, 128)
+    big = rng_rows(3, (nb * 64, hkv, 128), "bf16").double().numpy() * 2.0 ** 16
+    orc.store(big, *pages.np[1], np.arange(nb * 64), False)
+    q = (rng_rows(13, (n, hq, 128), "bf16") * up).cuda()
+    scale = 128 ** -0.5 / up
+    out = flash_attn_with_kvcache(q[None], *pages.gpu(), cache_seqlens=_int([90]),
+                                  block_table=_int(tables), softmax_scale=scale, causal=True)
+    ref, size = _reference(q, pages, tables, [n], [90], scale)
+    assert_close(out[0], ref, size, "bf16", "fp4 far queries")
+
+
+def test_chunks_do_not_see_what_is_not_finite_behind_the_mask():
+    n, lens = 70, [100]
+    tables, nb = tables_of(lens, 64, 4)
+    pages = Pages(7, nb, 64, 2, 128)
+    q = rng_rows(1, (n, 4, 128), "bf16").cuda()
+    ref, size = _reference(q, pages, tables, [n], lens, 128 ** -0.5)
+    for i in range(2):                                # key 90: head 0's key, head 1's value
+        pages.np[i][1][tables[0][1], i, 2, 90 - 64] = np.nan
+    out = flash_attn_with_kvcache(q[None], *pages.gpu(), cache_seqlens=_int(lens),
+                                  block_table=_int(tables), causal=True)[0]
+    sees = 90 - (100 - n)                             # the first query that sees it
+    assert torch.isnan(out[sees:]).all()
+    assert_close(out[:sees], ref[:sees], size[:sees], "bf16", "fp4 chunk, masked NaN")
+
+
+def test_a_batch_larger_than_the_pages_goes_in_parts():
+    """Tables of 16384 tokens: 64 MiB of f16 keys and values for a sequence, so 8 at a time."""
+    lens, n = [40, 300, 17, 90, 33, 50, 64, 65, 129, 200, 35], 70
+    tables, nb = tables_of(lens, 256, 4)
+    pages = Pages(7, nb, 256, 8, 128)
+    wide = np.full((len(lens), 64), -1, np.int32)
+    wide[:, :tables.shape[1]] = tables
+    q = rng_rows(1, (len(lens), n, 16, 128), "bf16").cuda()
+    say("fp4 chunks in parts")
+    out = flash_attn_with_kvcache(q, *pages.gpu(), cache_seqlens=_int(lens), block_table=_int(wide),
+                                  causal=True)
+    ref, size = _reference(q.flatten(0, 1), pages, tables, [n] * len(lens), lens, 128 ** -0.5)
+    assert_close(out, ref, size, "bf16", "fp4 parts of a batch")
+
+
+def test_a_captured_chunk_follows_its_inputs():
+    lens, n = [100, 160], 70
+    tables, nb = tables_of([160] * 2, 64, 3)
+    pages = Pages(7, nb, 64, 2, 128)
+    q, keys = rng_rows(1, (2, n, 4, 128), "bf16").cuda(), _int(lens)
+    call = lambda: flash_attn_with_kvcache(q, *gpu, cache_seqlens=keys, block_table=bt, causal=True)
+    gpu, bt = pages.gpu(), _int(tables)
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for i, now in enumerate([lens, [60, 71], [160, 160], lens]):
+        q.copy_(rng_rows(20 + i, (2, n, 4, 128), "bf16"))
+        keys.copy_(_int(now))
+        graph.replay()
+        eager = call()
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager)
+        ref, size = _reference(q.flatten(0, 1), pages, tables, [n] * 2, now, 128 ** -0.5)
+        assert_close(out, ref, size, "bf16", f"fp4 chunk replay {i}")
 
 
 def test_queries_and_outputs_with_strides():
