@@ -34,6 +34,7 @@ constexpr int kMaxBatch = 2048;
 typedef __attribute__((address_space(4))) const int32_t const_i32;
 typedef __attribute__((address_space(3))) void* lds_ptr;
 typedef int i32x2 __attribute__((ext_vector_type(2)));
+typedef NvkElt<true>::vec8 vec8h;
 
 struct AttnArgs {
   const uint16_t* q;
@@ -45,7 +46,9 @@ struct AttnArgs {
   const int32_t* block_tables;
   int64_t bt_stride;
   int batch, n_query, max_tiles, cap, block_size, num_blocks;
+  int bs_shift;          // log2 of block_size, or -1
   int num_kv_heads, G;
+  uint32_t g_inverse;    // ceil(2^32 / G): rows (below 2^27) / G as a high product (G > 1)
   float scale_log2;
   uint16_t* out;
   int64_t out_stride_tok, out_stride_head;
@@ -114,15 +117,29 @@ __device__ int unit_prefix(const AttnArgs& a, int* s_cs, int* s_wsum) {
   return total;
 }
 
-__device__ __forceinline__ int64_t active_waves(int64_t T, int64_t P) {
-  return T < P ? (T < 1 ? 1 : T) : P;
-}
-__device__ __forceinline__ int64_t range_begin(int64_t w, int64_t T, int64_t P) { return w * T / P; }
-__device__ __forceinline__ int64_t chunk_owner(int64_t c, int64_t T, int64_t P) {
-  return ((c + 1) * P - 1) / T;
+// T chunks over P waves: the first T % P waves take one more than the others.
+struct Split {
+  int P, per, rem;
+  __device__ __forceinline__ int begin(int w) const { return w * per + (w < rem ? w : rem); }
+  __device__ __forceinline__ int owner(int c) const {  // of chunk c
+    const int big = rem * (per + 1);
+    return c < big ? c / (per + 1) : rem + (c - big) / per;
+  }
+};
+__device__ __forceinline__ Split split_of(int T, int n_waves) {
+  Split x;
+  x.P = T < n_waves ? T : n_waves;
+  x.per = x.P ? T / x.P : 0;
+  x.rem = T - x.P * x.per;
+  return x;
 }
 
-// 16 bytes per lane from its own address straight into LDS: lane l writes [dst + 16 l, +16).
+// 16 bytes per lane straight into LDS: lane l writes [dst + 16 l, +16).  From base + the lane's
+// offset, or from the lane's own address.
+__device__ __forceinline__ void lds_load(const void* base, uint32_t offset, uint32_t dst) {
+  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1 nt"
+               :: "v"(offset), "s"(base), "s"(dst) : "memory", "m0");
+}
 __device__ __forceinline__ void lds_load(const void* src, uint32_t dst) {
   asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off nt"
                :: "v"(src), "s"(dst) : "memory", "m0");
@@ -140,6 +157,17 @@ __device__ __forceinline__ float max_xor16(float x) {
   const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
+// (p0, p1) times a pair of f16 scales, each product rounded once to f16: v_fma_mixlo / mixhi_f16,
+// which take the scales as they are.  (The empty asm keeps the two roundings apart: a pair of them
+// becomes two conversions of the scales, two f32 products and one conversion.)
+__device__ __forceinline__ uint32_t times_scales(float p0, float p1, uint32_t scales) {
+  typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+  const h2 s = __builtin_bit_cast(h2, scales);
+  _Float16 lo = (_Float16)fmaf(p0, (float)s[0], 0.f);
+  asm("" : "+v"(lo));
+  const h2 d = {lo, (_Float16)fmaf(p1, (float)s[1], 0.f)};
+  return __builtin_bit_cast(uint32_t, d);
+}
 
 template <int HD>
 struct KeyVec;
@@ -153,7 +181,12 @@ struct KeyVec<64> {
 };
 
 // ONEPAGE: pages of a multiple of 64 keys, so that a chunk lies in one; else of a multiple of 16.
-template <int HD, bool F16, bool ONEPAGE>
+// FEW: steps of at most 16 / NG rows per kv head (NG = D / 32 groups), e.g. the decode of up to 4
+// heads of 128.  16 columns are then a row's NG groups: column (row, group) holds the query in
+// that group's dimensions and zeros elsewhere, so that the MFMAs of all steps add up to a group's
+// own sum.  One product with the scale per score, not NG, and NG lanes add up; and a lane needs
+// P vs of its own group only, whose dimensions alone are kept of its output.
+template <int HD, bool F16, bool ONEPAGE, bool FEW>
 __global__ __launch_bounds__(64 * kWavesPerWG, 2) void fp4_attention_kernel(AttnArgs a) {
   using E = NvkElt<F16>;
   typedef typename E::vec8 vec8;
@@ -164,6 +197,7 @@ __global__ __launch_bounds__(64 * kWavesPerWG, 2) void fp4_attention_kernel(Attn
   constexpr int kBuf = kVBytes + 1024;     // and its scales (D = 64 uses half of the 1024)
   constexpr int kBlk = ONEPAGE ? 1 : 4;    // pages looked up per chunk
   constexpr int kRec = HD + 4;
+  constexpr int NS = FEW ? 1 : NG;         // groups whose scales a lane needs
   __shared__ __attribute__((aligned(1024))) uint8_t lds[kWavesPerWG * 2 * kBuf];
   __shared__ int s_cs[kMaxBatch + 1];
   __shared__ int s_wsum[kWavesPerWG];
@@ -180,12 +214,11 @@ __global__ __launch_bounds__(64 * kWavesPerWG, 2) void fp4_attention_kernel(Attn
         *reinterpret_cast<int2*>(a.desc + 2 * (int64_t)e) = make_int2(-1, -1);
     }
   }
-  const int64_t T = (int64_t)Hkv * S;
-  const int64_t P = active_waves(T, a.n_waves);
+  const Split sp = split_of(uniform(Hkv * S), a.n_waves);
   const int wave = uniform(tid >> 6);
-  const int64_t w = (int64_t)blockIdx.x * kWavesPerWG + wave;
-  if (w >= P || T == 0) return;
-  const int64_t c0 = range_begin(w, T, P), c1 = range_begin(w + 1, T, P);
+  const int w = blockIdx.x * kWavesPerWG + wave;
+  if (w >= sp.P) return;
+  const int c0 = sp.begin(w), c1 = sp.begin(w + 1);
   if (c0 >= c1) return;
 
   // position: sequence s, kv head, tile, chunk k of n
@@ -194,11 +227,11 @@ __global__ __launch_bounds__(64 * kWavesPerWG, 2) void fp4_attention_kernel(Attn
   int n = uniform(chunks_of(sq)), tiles = uniform(tiles_of(a, sq));
   int kvh, tile, k;
   {
-    int64_t rr = c0 - (int64_t)Hkv * s_cs[s];
-    kvh = uniform((int)(rr / ((int64_t)tiles * n)));
-    rr -= (int64_t)kvh * tiles * n;
-    tile = uniform((int)(rr / n));
-    k = uniform((int)(rr % n));
+    const int rr = c0 - Hkv * uniform(s_cs[s]);
+    const int unit = uniform(rr / n);
+    k = uniform(rr - unit * n);
+    kvh = uniform(unit / tiles);
+    tile = uniform(unit - kvh * tiles);
   }
   bool started_here = k == 0;
 
@@ -216,10 +249,16 @@ __global__ __launch_bounds__(64 * kWavesPerWG, 2) void fp4_attention_kernel(Attn
   const int sl = HD == 128 ? lane : lane & 31;
   const bool s_is_v = sl >= 32 * NG / 4;
   const int s_grp = (sl >> 3) & (NG - 1), s_key = 8 * (sl & 7);
+  const char* s_base = reinterpret_cast<const char*>(s_is_v ? a.v_scale : a.k_scale) +
+                       2 * (s_grp * a.block_size + (ONEPAGE ? s_key : s_key & 15));
+  const uint32_t k_off = (uint32_t)((ONEPAGE ? 16 * (r >> 2) : 0) + (r & 3)) * RB + g * (RB / 4);
+  const uint32_t v_off = (uint32_t)vrow * RB + vbyte;
+  const uint32_t head_bytes = (uint32_t)a.block_size * RB;        // a (page, head)'s codes
+  const uint64_t page_bytes = (uint64_t)head_bytes * Hkv;
 
-  // Where a chunk lies: the index of its (16-key blocks') first row, and of the same row's scale.
+  // Byte offsets of a chunk's (16-key blocks') first row of codes, and of the same row's scales.
   struct Where {
-    int64_t row[kBlk], srow[kBlk];
+    uint64_t row[kBlk], scale[kBlk];
   };
   auto locate = [&](const Seq& x, int ss, int hh, int kk) {
     Where p;
@@ -228,45 +267,47 @@ __global__ __launch_bounds__(64 * kWavesPerWG, 2) void fp4_attention_kernel(Attn
     for (int b = 0; b < kBlk; ++b) {
       int key = kk * kCK + 16 * b;
       if (key >= x.keys) key = kk * kCK;  // a block past the keys: any block, nothing of it counts
-      const int logical = key / a.block_size;
+      const int logical = a.bs_shift >= 0 ? key >> a.bs_shift : key / a.block_size;
       int page = bt[logical];
       if (page < 0 || page >= a.num_blocks) page = 0;
-      const int64_t head = (int64_t)page * Hkv + hh;
-      const int off = key - logical * a.block_size;
-      p.row[b] = head * a.block_size + off;
-      p.srow[b] = head * NG * a.block_size + off;
+      const uint32_t off = (uint32_t)(key - logical * a.block_size);
+      const uint64_t head = (uint64_t)(uint32_t)page * page_bytes + (uint64_t)(uint32_t)hh * head_bytes;
+      p.row[b] = head + off * RB;
+      p.scale[b] = (head >> 3) + off * 2;  // 2 bytes of scale per 16 of codes
     }
     return p;
   };
-  auto pick = [](const int64_t* v, int i) {  // v[i] of a lane's block i
+  auto pick = [](const uint64_t* v, int i) {  // v[i] of a lane's block i
     if constexpr (kBlk == 1) return v[0];
     else return i & 2 ? (i & 1 ? v[3] : v[2]) : (i & 1 ? v[1] : v[0]);
   };
   auto issue = [&](const Where& p, uint32_t buf, kvec (&kraw)[4]) {
-    const int64_t krow = kBlk == 1 ? p.row[0] + 16 * (r >> 2) : pick(p.row, r >> 2);
-    const uint8_t* kp = a.k_data + (krow + (r & 3)) * RB + g * (RB / 4);
+    const uint8_t* kp = a.k_data + (kBlk == 1 ? p.row[0] : pick(p.row, r >> 2)) + k_off;
 #pragma unroll
     for (int b = 0; b < 4; ++b)
       kraw[b] = __builtin_nontemporal_load(reinterpret_cast<const kvec*>(kp + 4 * b * RB));
 #pragma unroll
     for (int j = 0; j < kVBytes / 1024; ++j) {
-      const int row = kRowsPerLoad * j + vrow;  // of the chunk
-      const int64_t vr = kBlk == 1 ? p.row[0] + row : pick(p.row, row >> 4) + (row & 15);
-      lds_load(a.v_data + vr * RB + vbyte, buf + 1024 * j);
+      if constexpr (kBlk == 1) {
+        lds_load(a.v_data + p.row[0], v_off + 1024u * j, buf + 1024 * j);
+      } else {
+        const int row = kRowsPerLoad * j + vrow;  // of the chunk
+        lds_load(a.v_data + pick(p.row, row >> 4) + ((row & 15) * RB + vbyte), buf + 1024 * j);
+      }
     }
-    const int64_t sr = kBlk == 1 ? p.srow[0] + s_key : pick(p.srow, s_key >> 4) + (s_key & 15);
-    lds_load((s_is_v ? a.v_scale : a.k_scale) + sr + (int64_t)s_grp * a.block_size, buf + kVBytes);
+    lds_load(s_base + (kBlk == 1 ? p.scale[0] : pick(p.scale, s_key >> 4)), buf + kVBytes);
   };
 
   // per-group state
   vec8 qf[NG];
   nvk_f32x4 acc[HD / 16];
-  float m_run = -INFINITY, l_part = 0.f;
+  float m_run = -INFINITY, l_part[2] = {0.f, 0.f};
   int tok = 0, head = 0, row_limit = 0, full_limit = 0;
   bool row_valid = false;
+  const int row = FEW ? r / NG : r, grp = r & (NG - 1);  // this column's (FEW: and its group)
   auto start_group = [&]() {
-    const int rr = tile * kR + r;
-    tok = rr / a.G;
+    const int rr = tile * kR + row;
+    tok = a.G == 1 ? rr : (int)__umulhi((uint32_t)rr, a.g_inverse);
     head = kvh * a.G + rr - tok * a.G;
     row_valid = tok < sq.queries;
     const int diag = sq.raw_keys - sq.queries;
@@ -277,13 +318,13 @@ __global__ __launch_bounds__(64 * kWavesPerWG, 2) void fp4_attention_kernel(Attn
 #pragma unroll
     for (int i = 0; i < NG; ++i) {
       nvk_u32x4 v = {0u, 0u, 0u, 0u};
-      if (row_valid) v = *reinterpret_cast<const nvk_u32x4*>(qp + 32 * i);
+      if (row_valid && (!FEW || i == grp)) v = *reinterpret_cast<const nvk_u32x4*>(qp + 32 * i);
       qf[i] = __builtin_bit_cast(vec8, v);
     }
 #pragma unroll
     for (int d = 0; d < HD / 16; ++d) acc[d] = nvk_f32x4{0.f, 0.f, 0.f, 0.f};
     m_run = -INFINITY;
-    l_part = 0.f;
+    l_part[0] = l_part[1] = 0.f;
   };
 
   kvec kraw[4];
@@ -291,7 +332,7 @@ __global__ __launch_bounds__(64 * kWavesPerWG, 2) void fp4_attention_kernel(Attn
   start_group();
   uint32_t cur = 0;
 
-  for (int64_t c = c0;; ++c) {
+  for (int c = c0;; ++c) {
     // ---- the next chunk's position
     const bool last = c + 1 == c1;
     const bool group_end = k == n - 1;
@@ -325,18 +366,49 @@ __global__ __launch_bounds__(64 * kWavesPerWG, 2) void fp4_attention_kernel(Attn
     // ---- scores of keys 16 g + 4 b + i, row r
     const int kbase = k * kCK;
     nvk_f32x4 sc[4] = {};
+    auto scales = [&](int tensor, int i) {  // of this lane's 16 keys
+      return (const __attribute__((address_space(3))) nvk_f16x8*)(size_t)(
+          buf + kVBytes + (uint32_t)(128 * (NG * tensor + i) + 32 * g));
+    };
+    if constexpr (FEW) {
+      const auto* kp = scales(0, grp);
+      const nvk_f16x8 ks[2] = {kp[0], kp[1]};
 #pragma unroll
-    for (int i = 0; i < NG; ++i) {
-      const auto* sp = (const __attribute__((address_space(3))) nvk_f16x8*)(size_t)(
-          buf + kVBytes + 128 * i + 32 * g);
-      const nvk_f16x8 ks[2] = {sp[0], sp[1]};
+      for (int i = 0; i < NG; ++i)
 #pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        const nvk_f32x4 z = {0.f, 0.f, 0.f, 0.f};
-        const nvk_f32x4 t = E::mfma16x16x32(fp4_unpack<F16>(kraw[b][i]), qf[i], z);
+        for (int b = 0; b < 4; ++b)
+          sc[b] = E::mfma16x16x32(fp4_unpack<F16>(kraw[b][i]), qf[i], sc[b]);
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          sc[b][e] = fmaf(t[e], (float)ks[b >> 1][4 * (b & 1) + e], sc[b][e]);
+          sc[b][e] = fmaf(sc[b][e], (float)ks[b >> 1][4 * (b & 1) + e], 0.f);
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sc[b][e] += nvk_dpp<NVK_DPP_QP_XOR1>(sc[b][e]);
+      if constexpr (NG == 4) {
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[b][e] += nvk_dpp<NVK_DPP_QP_XOR2>(sc[b][e]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NG; ++i) {
+        const auto* kp = scales(0, i);
+        const nvk_f16x8 ks[2] = {kp[0], kp[1]};
+        nvk_f32x4 t[4];
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          const nvk_f32x4 z = {0.f, 0.f, 0.f, 0.f};
+          t[b] = E::mfma16x16x32(fp4_unpack<F16>(kraw[b][i]), qf[i], z);
+        }
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            sc[b][e] = fmaf(t[b][e], (float)ks[b >> 1][4 * (b & 1) + e], sc[b][e]);
       }
     }
 
@@ -349,16 +421,18 @@ __global__ __launch_bounds__(64 * kWavesPerWG, 2) void fp4_attention_kernel(Attn
 #pragma unroll
         for (int e = 0; e < 4; ++e) sc[b][e] = 4 * b + e < seen ? sc[b][e] : -INFINITY;
     }
-    float mx = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3]));
-#pragma unroll
-    for (int b = 1; b < 4; ++b)
-      mx = fmaxf(mx, fmaxf(fmaxf(sc[b][0], sc[b][1]), fmaxf(sc[b][2], sc[b][3])));
+    float mx = nvk_max3(nvk_max3(sc[0][0], sc[0][1], sc[0][2]),
+                        nvk_max3(sc[0][3], sc[1][0], sc[1][1]),
+                        nvk_max3(sc[1][2], sc[1][3], sc[2][0]));
+    mx = nvk_max3(nvk_max3(sc[2][1], sc[2][2], sc[2][3]), mx,
+                  nvk_max3(sc[3][0], sc[3][1], nvk_max3(sc[3][2], sc[3][3], sc[3][3])));
     mx = nvk_max_xor32(max_xor16(mx));
-    const float m_new = fmaxf(m_run, mx == -INFINITY ? -INFINITY : mx * a.scale_log2);
+    const float m_new = fmaxf(m_run, mx * a.scale_log2);
     const float moff = m_new == -INFINITY ? 0.f : m_new;
     if (__builtin_amdgcn_ballot_w64(m_new > m_run)) {
       const float alpha = nvk_fast_exp2(m_run - moff);  // 0 while nothing was visible
-      l_part *= alpha;
+      l_part[0] *= alpha;
+      l_part[1] *= alpha;
 #pragma unroll
       for (int d = 0; d < HD / 16; ++d) acc[d] *= alpha;
       m_run = m_new;
@@ -368,70 +442,90 @@ __global__ __launch_bounds__(64 * kWavesPerWG, 2) void fp4_attention_kernel(Attn
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         sc[b][e] = nvk_fast_exp2(fmaf(sc[b][e], a.scale_log2, -moff));
-        l_part += sc[b][e];
+        l_part[e & 1] += sc[b][e];
       }
 
     // ---- O^T += V^T (P vs)^T, one operand per group of dimensions
-    auto pv = [&](auto masked) {
+    vec8h pf[2];
 #pragma unroll
-      for (int i = 0; i < NG; ++i) {
-        const auto* sp = (const __attribute__((address_space(3))) nvk_f16x8*)(size_t)(
-            buf + kVBytes + 128 * NG + 128 * i + 32 * g);
-        nvk_f16x8 pf[2] = {sp[0], sp[1]};
+    for (int i = 0; i < NG; ++i) {
+      if (i < NS) {
+        const auto* vp = scales(1, FEW ? grp : i);
+        nvk_u32x4 vs[2] = {__builtin_bit_cast(nvk_u32x4, vp[0]), __builtin_bit_cast(nvk_u32x4, vp[1])};
+        if (!full) {
+          // a masked key's scale may be anything, what an earlier owner of the page left too
 #pragma unroll
-        for (int b = 0; b < 4; ++b)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int j = 4 * (b & 1) + e;
-            const float x = sc[b][e] * (float)pf[b >> 1][j];
-            // a masked key's scale may be anything, what an earlier owner of the page left too
-            pf[b >> 1][j] = (_Float16)(!decltype(masked)::value || 4 * b + e < seen ? x : 0.f);
+          for (int p = 0; p < 8; ++p) {
+            const int t = seen - 2 * p;
+            vs[p >> 2][p & 3] &= t >= 2 ? 0xffffffffu : t == 1 ? 0xffffu : 0u;
           }
+        }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const int d = 2 * i + h;
-          const i32x2 vc = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
-              (__attribute__((address_space(3))) i32x2*)(size_t)(buf + tr_row + 16 * (i ^ sw) +
-                                                                  8 * h));
-          acc[d] = NvkElt<true>::mfma16x16x32(fp4_unpack<true>((uint32_t)vc[0]), pf[0], acc[d]);
-          acc[d] = NvkElt<true>::mfma16x16x32(fp4_unpack<true>((uint32_t)vc[1]), pf[1], acc[d]);
+          nvk_u32x4 x;
+#pragma unroll
+          for (int p = 0; p < 4; ++p)
+            x[p] = times_scales(sc[2 * h + (p >> 1)][2 * (p & 1)], sc[2 * h + (p >> 1)][2 * (p & 1) + 1],
+                                vs[h][p]);
+          pf[h] = __builtin_bit_cast(vec8h, x);
         }
       }
-    };
-    if (full) pv(std::false_type{});
-    else pv(std::true_type{});
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int d = 2 * i + h;
+        const i32x2 vc = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
+            (__attribute__((address_space(3))) i32x2*)(size_t)(buf + tr_row + 16 * (i ^ sw) +
+                                                                8 * h));
+        acc[d] = NvkElt<true>::mfma16x16x32(fp4_unpack<true>((uint32_t)vc[0]), pf[0], acc[d]);
+        acc[d] = NvkElt<true>::mfma16x16x32(fp4_unpack<true>((uint32_t)vc[1]), pf[1], acc[d]);
+      }
+    }
 
     // ---- the group's or the range's end
     if (group_end || last) {
-      const float l_tot = nvk_sum_xor32(sum_xor16(l_part));
+      const float l_tot = nvk_sum_xor32(sum_xor16(l_part[0] + l_part[1]));
+      // the d blocks that this lane's column is kept of: FEW: those of its group
+      constexpr int kKeep = FEW ? 2 : HD / 16;
+      nvk_f32x4 o[kKeep];
+#pragma unroll
+      for (int j = 0; j < kKeep; ++j) {
+        o[j] = acc[j];
+        if constexpr (FEW) {
+#pragma unroll
+          for (int i = 1; i < NG; ++i)
+            if (grp == i) o[j] = acc[2 * i + j];
+        }
+      }
+      const int d0 = (FEW ? 32 * grp : 0) + 4 * g;  // dimension of o[0][0]
       if (group_end && started_here) {
         if (row_valid) {
           const float inv = l_tot == 0.f ? 0.f : 1.f / l_tot;
           uint16_t* op = a.out + (int64_t)(sq.row0 + tok) * a.out_stride_tok +
-                         (int64_t)head * a.out_stride_head + 4 * g;
+                         (int64_t)head * a.out_stride_head + d0;
 #pragma unroll
-          for (int d = 0; d < HD / 16; ++d) {
+          for (int j = 0; j < kKeep; ++j) {
             nvk_u32x2 wv;
-            wv.x = E::pack2(acc[d][0] * inv, acc[d][1] * inv);
-            wv.y = E::pack2(acc[d][2] * inv, acc[d][3] * inv);
-            *reinterpret_cast<nvk_u32x2*>(op + 16 * d) = wv;
+            wv.x = E::pack2(o[j][0] * inv, o[j][1] * inv);
+            wv.y = E::pack2(o[j][2] * inv, o[j][3] * inv);
+            *reinterpret_cast<nvk_u32x2*>(op + 16 * j) = wv;
           }
         }
       } else if (row_valid) {  // the merge reads the valid rows only
-        float* rec = a.rec + ((w * 2 + (started_here ? 0 : 1)) * a.rec_rows + r) * (int64_t)kRec;
+        float* rec =
+            a.rec + ((int64_t)(w * 2 + (started_here ? 0 : 1)) * a.rec_rows + row) * kRec;
 #pragma unroll
-        for (int d = 0; d < HD / 16; ++d)
-          *reinterpret_cast<nvk_f32x4*>(rec + 16 * d + 4 * g) = acc[d];
-        if (g == 0) {
+        for (int j = 0; j < kKeep; ++j)
+          *reinterpret_cast<nvk_f32x4*>(rec + d0 + 16 * j) = o[j];
+        if (g == 0 && (!FEW || grp == 0)) {
           rec[HD] = m_run;
           rec[HD + 1] = l_tot;
         }
       }
       if (lane == 0) {
-        const int64_t first = (int64_t)Hkv * s_cs[s] + ((int64_t)kvh * tiles + tile) * n;
-        const int p1 = (int)chunk_owner(first, T, P), p2 = (int)chunk_owner(first + n - 1, T, P);
+        const int first = Hkv * s_cs[s] + (kvh * tiles + tile) * n;
         const int64_t e = ((int64_t)s * Hkv + kvh) * a.max_tiles + tile;
-        *reinterpret_cast<int2*>(a.desc + 2 * e) = make_int2(p1, p2);
+        *reinterpret_cast<int2*>(a.desc + 2 * e) =
+            make_int2(sp.owner(first), sp.owner(first + n - 1));
       }
       if (last) return;
       s = ns;
@@ -560,8 +654,9 @@ bool plan_of(int batch, int max_queries, int num_q_heads, int num_kv_heads, int 
   const int64_t rows = (int64_t)max_queries * G;
   const int64_t chunks = ((int64_t)max_blocks * block_size + kCK - 1) / kCK;
   const int64_t tiles = (rows + kR - 1) / kR;
-  if (tiles * num_kv_heads * 8 > INT32_MAX || chunks > INT32_MAX / kCK ||
-      tiles * chunks > INT32_MAX / batch || tiles * num_kv_heads > INT32_MAX / batch)
+  if (rows >= 1 << 27 || tiles * num_kv_heads * 8 > INT32_MAX || chunks > INT32_MAX / kCK ||
+      tiles * chunks > INT32_MAX / batch / num_kv_heads ||
+      (int64_t)block_size * num_kv_heads * head_dim > INT32_MAX)
     return false;
   p.max_tiles = (int)tiles;
   p.rec_rows = (int)(rows < kR ? rows : kR);
@@ -577,10 +672,14 @@ bool plan_of(int batch, int max_queries, int num_q_heads, int num_kv_heads, int 
 template <int HD, bool F16>
 int launch(const AttnArgs& a, hipStream_t s) {
   const dim3 grid(a.n_waves / kWavesPerWG), block(64 * kWavesPerWG);
-  if (a.block_size % kCK == 0)
-    hipLaunchKernelGGL((fp4_attention_kernel<HD, F16, true>), grid, block, 0, s, a);
-  else
-    hipLaunchKernelGGL((fp4_attention_kernel<HD, F16, false>), grid, block, 0, s, a);
+  const auto main = [&](auto one, auto few) {
+    hipLaunchKernelGGL((fp4_attention_kernel<HD, F16, decltype(one)::value, decltype(few)::value>),
+                       grid, block, 0, s, a);
+  };
+  const std::true_type yes;
+  const std::false_type no;
+  if (a.n_query * a.G <= kR / (HD / kFp4Group)) a.block_size % kCK ? main(no, yes) : main(yes, yes);
+  else a.block_size % kCK ? main(no, no) : main(yes, no);
   const int st = nvk_launch_status();
   if (st != NVK_OK) return st;
   const dim3 mgrid(a.num_kv_heads * a.max_tiles * ((a.rec_rows + 1) / 2), a.batch);
@@ -772,9 +871,11 @@ extern "C" int nvk_fp4_attention(const void* q, int64_t q_stride_tok, int64_t q_
   a.max_tiles = p.max_tiles;
   a.cap = max_blocks * block_size;
   a.block_size = block_size;
+  a.bs_shift = nvk_log2_exact(block_size);
   a.num_blocks = num_blocks;
   a.num_kv_heads = num_kv_heads;
   a.G = num_q_heads / num_kv_heads;
+  a.g_inverse = a.G > 1 ? (uint32_t)((((uint64_t)1 << 32) + a.G - 1) / a.G) : 0;
   a.scale_log2 = scale * NVK_LOG2E;
   a.out = static_cast<uint16_t*>(out);
   a.out_stride_tok = out_stride_tok;
