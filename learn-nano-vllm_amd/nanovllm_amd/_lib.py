@@ -223,9 +223,16 @@ def workspace(device: torch.device, nbytes: int) -> torch.Tensor | None:
     if nbytes <= 0:
         return None
     with on_device(device):
-        if torch.cuda.is_current_stream_capturing():
-            return torch.empty(nbytes, dtype=torch.uint8, device=device)
-    key = (device.index, stream_ptr(device))
+        return workspace_on(device, stream_ptr(device), nbytes)
+
+
+def workspace_on(device: torch.device, stream: int, nbytes: int) -> torch.Tensor | None:
+    """``workspace`` where `device` is current and `stream` its current stream."""
+    if nbytes <= 0:
+        return None
+    if torch.cuda.is_current_stream_capturing():
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+    key = (device.index, stream)
     buf = _workspaces.get(key)
     if buf is None or buf.numel() < nbytes:
         buf = torch.empty(nbytes, dtype=torch.uint8, device=device)

@@ -258,22 +258,23 @@ def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, rotary_cos=None
         raise _lib.NvkError("q must be [batch, seqlen_q, heads, head_dim]")
     b, sq, hq, d = q.shape
     fp4 = isinstance(k_cache, Fp4Cache) or isinstance(v_cache, Fp4Cache)
-    dev = _lib.require_gpu(q) if fp4 else _lib.require_gpu(q, k_cache, v_cache)
+    dev = q.device if fp4 else _lib.require_gpu(q, k_cache, v_cache)
     if cache_seqlens is None:
         raise NotImplementedError("nanovllm_amd: cache_seqlens is required")
     if isinstance(cache_seqlens, int):
         cache_seqlens = torch.full((b,), cache_seqlens, dtype=torch.int32, device=dev)
     if block_table is None:
         block_table = torch.arange(b, dtype=torch.int32, device=dev).view(b, 1)
+    if fp4:
+        if sq > 1 and not causal:
+            raise NotImplementedError("nanovllm_amd: seqlen_q > 1 needs causal=True")
+        return fp4_attention(q, k_cache, v_cache, cache_seqlens, block_table, softmax_scale,
+                             max_seqlen_q=sq)
     if sq == 1:
         out = paged_decode(q[:, 0], k_cache, v_cache, cache_seqlens, block_table, softmax_scale)
         return out.view(b, 1, hq, d)
     if not causal:
         raise NotImplementedError("nanovllm_amd: seqlen_q > 1 needs causal=True")
-    if fp4:
-        out = fp4_attention(q.reshape(b * sq, hq, d), k_cache, v_cache, cache_seqlens, block_table,
-                            softmax_scale, max_seqlen_q=sq)
-        return out.view(b, sq, hq, d)
     lens = _int32(cache_seqlens)
     out = _verify(q, k_cache, v_cache, lens, block_table, softmax_scale)
     if out is not None:

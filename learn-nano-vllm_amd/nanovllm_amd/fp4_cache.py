@@ -9,6 +9,7 @@ no such cache.
 """
 from __future__ import annotations
 
+import functools
 from typing import NamedTuple
 
 import torch
@@ -52,29 +53,51 @@ class Fp4Cache(NamedTuple):
 
 def _check_caches(k_cache, v_cache):
     """(num_blocks, block_size, num_kv_heads, head_dim) of a pair of caches."""
-    for c in (k_cache, v_cache):
-        if not isinstance(c, Fp4Cache):
-            raise _lib.NvkError("k_cache and v_cache must both be Fp4Cache")
-        if (c.data.dim() != 4 or c.scale.dim() != 4 or c.data.dtype != torch.uint8
-                or c.scale.dtype != torch.float16 or not c.data.is_contiguous()
-                or not c.scale.is_contiguous()):
-            raise _lib.NvkError("Fp4Cache must be contiguous uint8 [num_blocks, Hkv, block_size, "
-                                "D / 2] and float16 [num_blocks, Hkv, D / 32, block_size]")
-    nb, hkv, bs, half = k_cache.data.shape
-    if (k_cache.data.shape != v_cache.data.shape or half not in (32, 64) or bs % 16
-            or k_cache.scale.shape != (nb, hkv, half // 16, bs)
-            or v_cache.scale.shape != k_cache.scale.shape):
+    if not (isinstance(k_cache, Fp4Cache) and isinstance(v_cache, Fp4Cache)):
+        raise _lib.NvkError("k_cache and v_cache must both be Fp4Cache")
+    (kd, ks), (vd, vs) = k_cache, v_cache
+    shape = kd.shape
+    if len(shape) != 4:
+        raise _lib.NvkError("Fp4Cache data must be [num_blocks, Hkv, block_size, D / 2]")
+    nb, hkv, bs, half = shape
+    if (kd.dtype != torch.uint8 or vd.dtype != torch.uint8 or ks.dtype != torch.float16
+            or vs.dtype != torch.float16 or not kd.is_contiguous() or not vd.is_contiguous()
+            or not ks.is_contiguous() or not vs.is_contiguous()):
+        raise _lib.NvkError("Fp4Cache must be contiguous uint8 [num_blocks, Hkv, block_size, D / 2] "
+                            "and float16 [num_blocks, Hkv, D / 32, block_size]")
+    if ((half != 64 and half != 32) or bs % 16 or vd.shape != shape
+            or ks.shape != (nb, hkv, half // 16, bs) or vs.shape != ks.shape):
         raise _lib.NvkError("Fp4Cache shapes disagree, or head_dim is not 128 or 64, or block_size "
                             "not a multiple of 16")
     return nb, bs, hkv, 2 * half
 
 
+def _device(k_cache, v_cache, *tensors):
+    """The GPU that the caches and the tensors are on (they have to share one)."""
+    first = k_cache.data
+    dev = first.device
+    for t in (k_cache.scale, *v_cache, *tensors):
+        if t.device != dev:
+            _lib.require_gpu(first, t)    # raises
+    if not first.is_cuda:
+        _lib.require_gpu(first)           # raises
+    return dev
+
+
+_ROWS = {torch.bfloat16: _lib.NVK_DTYPE_BF16, torch.float16: _lib.NVK_DTYPE_F16}
+
+
 def _rows_dtype(dtype: torch.dtype) -> int:
-    if dtype == torch.bfloat16:
-        return _lib.NVK_DTYPE_BF16
-    if dtype == torch.float16:
-        return _lib.NVK_DTYPE_F16
-    raise _lib.NvkError(f"a 4-bit cache takes and gives bfloat16 and float16 rows, got {dtype}")
+    code = _ROWS.get(dtype)
+    if code is None:
+        raise _lib.NvkError(f"a 4-bit cache takes and gives bfloat16 and float16 rows, got {dtype}")
+    return code
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(*sizes: int) -> int:
+    """nvk_fp4_attention_workspace_size, a function of its sizes alone."""
+    return _lib.load().nvk_fp4_attention_workspace_size(*sizes)
 
 
 def fp4_store(key: torch.Tensor, value: torch.Tensor, k_cache: Fp4Cache, v_cache: Fp4Cache,
@@ -85,18 +108,19 @@ def fp4_store(key: torch.Tensor, value: torch.Tensor, k_cache: Fp4Cache, v_cache
     dtype = _rows_dtype(key.dtype)
     N = key.shape[0]
     assert key.shape == value.shape == (N, hkv, d) and key.dtype == value.dtype
-    assert key.stride(-1) == 1 and value.stride(-1) == 1
-    assert key.stride(1) == d and value.stride(1) == d
+    (ks, kh, k1), (vs, vh, v1) = key.stride(), value.stride()
+    assert k1 == 1 and v1 == 1
+    assert kh == d and vh == d
     assert slot_mapping.numel() == N
-    dev = _lib.require_gpu(key, value, *k_cache, *v_cache, slot_mapping)
+    dev = _device(k_cache, v_cache, key, value, slot_mapping)
     slots = _lib.int32(slot_mapping)
     with _lib.on_device(dev):
         code = _lib.load().nvk_fp4_store(
-            key.data_ptr(), key.stride(0), value.data_ptr(), value.stride(0),
-            k_cache.data.data_ptr(), k_cache.scale.data_ptr(), v_cache.data.data_ptr(),
-            v_cache.scale.data_ptr(), slots.data_ptr(), N, hkv, d, bs, nb, dtype,
-            _lib.stream_ptr(dev))
-    _lib.check(code)
+            key.data_ptr(), ks, value.data_ptr(), vs, k_cache.data.data_ptr(),
+            k_cache.scale.data_ptr(), v_cache.data.data_ptr(), v_cache.scale.data_ptr(),
+            slots.data_ptr(), N, hkv, d, bs, nb, dtype, _lib.stream_ptr(dev))
+    if code:
+        _lib.check(code)
 
 
 def load_kvcache(k_cache: Fp4Cache, v_cache: Fp4Cache, slot_mapping: torch.Tensor,
@@ -106,16 +130,18 @@ def load_kvcache(k_cache: Fp4Cache, v_cache: Fp4Cache, slot_mapping: torch.Tenso
     was rounded.  A slot outside the cache (-1) gives zeros."""
     nb, bs, hkv, d = _check_caches(k_cache, v_cache)
     code = _rows_dtype(dtype)
-    dev = _lib.require_gpu(*k_cache, *v_cache, slot_mapping)
-    slots = _lib.int32(slot_mapping).view(-1)
+    dev = _device(k_cache, v_cache, slot_mapping)
+    slots = _lib.int32(slot_mapping)
     N = slots.numel()
-    key, value = (torch.empty(N, hkv, d, dtype=dtype, device=dev) for _ in range(2))
+    key = torch.empty((N, hkv, d), dtype=dtype, device=dev)
+    value = torch.empty_like(key)
     with _lib.on_device(dev):
         st = _lib.load().nvk_fp4_load(
             k_cache.data.data_ptr(), k_cache.scale.data_ptr(), v_cache.data.data_ptr(),
             v_cache.scale.data_ptr(), slots.data_ptr(), N, hkv, d, bs, nb, key.data_ptr(), hkv * d,
             value.data_ptr(), hkv * d, code, _lib.stream_ptr(dev))
-    _lib.check(st)
+    if st:
+        _lib.check(st)
     return key, value
 
 
@@ -124,40 +150,58 @@ def fp4_attention(q: torch.Tensor, k_cache: Fp4Cache, v_cache: Fp4Cache, seqlens
                   max_seqlen_q: int = 1, max_seqlen_k: int | None = None,
                   out: torch.Tensor | None = None) -> torch.Tensor:
     """Causal attention of q [tokens, Hq, D] over 4-bit caches.  Without ``cu_seqlens_q`` every
-    sequence has ``max_seqlen_q`` queries and ``seqlens_k`` [B] keys; with it both are prefix sums
-    [B + 1].  The queries are the last of their sequence's keys.  ``max_seqlen_k`` bounds the keys of
-    a sequence (None: what the block table holds).  Returns [tokens, Hq, D] (or fills ``out``)."""
+    sequence has ``max_seqlen_q`` queries and ``seqlens_k`` [B] keys (q may then be
+    [B, max_seqlen_q, Hq, D]); with it both are prefix sums [B + 1].  The queries are the last of
+    their sequence's keys.  ``max_seqlen_k`` bounds the keys of a sequence (None: what the block
+    table holds).  Returns a tensor like q (or fills ``out``)."""
     nb, bs, hkv, d = _check_caches(k_cache, v_cache)
-    dev = _lib.require_gpu(q, *k_cache, *v_cache, seqlens_k, block_table, cu_seqlens_q)
     dtype = _rows_dtype(q.dtype)
-    if q.dim() != 3 or q.stride(-1) != 1 or q.shape[2] != d:
-        raise _lib.NvkError("q must be [tokens, heads, head_dim] with unit last stride and the "
-                            "caches' head_dim")
-    tq, hq, _ = q.shape
+    shape, strides = q.shape, q.stride()
+    if len(shape) == 4 and cu_seqlens_q is None and out is None and shape[1] == max_seqlen_q:
+        if shape[1] != 1 and strides[0] != shape[1] * strides[1]:
+            q = q.contiguous()
+            strides = q.stride()
+        tq, (row, head, last) = shape[0] * shape[1], strides[1:]
+        if shape[1] == 1:
+            row = strides[0]
+    elif len(shape) == 3:
+        tq, (row, head, last) = shape[0], strides
+    else:
+        raise _lib.NvkError("q must be [tokens, heads, head_dim]")
+    if last != 1 or shape[-1] != d:
+        raise _lib.NvkError("q must have unit last stride and the caches' head_dim")
+    hq = shape[-2]
     lens, bt = _lib.int32(seqlens_k), _lib.int32(block_table)
     cu_q = None if cu_seqlens_q is None else _lib.int32(cu_seqlens_q)
-    batch = lens.numel() - (cu_q is not None)
-    if cu_q is not None and cu_q.numel() != lens.numel():
-        raise _lib.NvkError("cu_seqlens_q and cu_seqlens_k disagree on the batch size")
-    if cu_q is None and batch * max_seqlen_q != tq:
+    batch = lens.numel()
+    if cu_q is not None:
+        if cu_q.numel() != batch:
+            raise _lib.NvkError("cu_seqlens_q and cu_seqlens_k disagree on the batch size")
+        batch -= 1
+    elif batch * max_seqlen_q != tq:
         raise _lib.NvkError("q and cache_seqlens disagree on the batch size")
     if bt.dim() != 2 or bt.shape[0] != batch:
         raise _lib.NvkError("block_table must be [batch, max_blocks]")
+    dev = _device(k_cache, v_cache, q, lens, bt, *(() if cu_q is None else (cu_q,)))
     if out is None:
-        out = torch.empty((tq, hq, d), dtype=q.dtype, device=dev)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or out.stride(-1) != 1:
-        raise _lib.NvkError("out must be like q, with unit last stride")
-    scale = float(softmax_scale) if softmax_scale is not None else d ** -0.5
-    lib = _lib.load()
+        out = torch.empty_like(q) if q.is_contiguous() else torch.empty(shape, dtype=q.dtype,
+                                                                        device=dev)
+        out_row, out_head = hq * d, d
+    else:
+        if out.shape != shape or out.dtype != q.dtype or out.device != dev or out.stride(-1) != 1:
+            raise _lib.NvkError("out must be like q, with unit last stride")
+        out_row, out_head = out.stride()[:2]
+    scale = d ** -0.5 if softmax_scale is None else float(softmax_scale)
     mq, mk, width = int(max_seqlen_q), int(max_seqlen_k or 0), bt.shape[1]
-    ws_bytes = lib.nvk_fp4_attention_workspace_size(batch, mq, mk, hq, hkv, d, bs, width)
-    ws = _lib.workspace(dev, ws_bytes)
+    ws_bytes = _workspace_bytes(batch, mq, mk, hq, hkv, d, bs, width)
     with _lib.on_device(dev):
-        code = lib.nvk_fp4_attention(
-            q.data_ptr(), q.stride(0), q.stride(1), tq, k_cache.data.data_ptr(),
-            k_cache.scale.data_ptr(), v_cache.data.data_ptr(), v_cache.scale.data_ptr(),
-            _lib.ptr(cu_q), lens.data_ptr(), batch, mq, mk, bt.data_ptr(), bt.stride(0), width, bs,
-            nb, hq, hkv, d, scale, out.data_ptr(), out.stride(0), out.stride(1), _lib.ptr(ws),
-            ws_bytes, dtype, _lib.stream_ptr(dev))
-    _lib.check(code)
+        stream = _lib.stream_ptr(dev)
+        ws = _lib.workspace_on(dev, stream, ws_bytes)
+        code = _lib.load().nvk_fp4_attention(
+            q.data_ptr(), row, head, tq, k_cache.data.data_ptr(), k_cache.scale.data_ptr(),
+            v_cache.data.data_ptr(), v_cache.scale.data_ptr(), _lib.ptr(cu_q), lens.data_ptr(),
+            batch, mq, mk, bt.data_ptr(), bt.stride(0), width, bs, nb, hq, hkv, d, scale,
+            out.data_ptr(), out_row, out_head, _lib.ptr(ws), ws_bytes, dtype, stream)
+    if code:
+        _lib.check(code)
     return out
