@@ -57,30 +57,31 @@ def _check_caches(k_cache, v_cache):
         raise _lib.NvkError("k_cache and v_cache must both be Fp4Cache")
     (kd, ks), (vd, vs) = k_cache, v_cache
     shape = kd.shape
-    if len(shape) != 4:
-        raise _lib.NvkError("Fp4Cache data must be [num_blocks, Hkv, block_size, D / 2]")
-    nb, hkv, bs, half = shape
-    if (kd.dtype != torch.uint8 or vd.dtype != torch.uint8 or ks.dtype != torch.float16
-            or vs.dtype != torch.float16 or not kd.is_contiguous() or not vd.is_contiguous()
-            or not ks.is_contiguous() or not vs.is_contiguous()):
+    if ((kd.dtype, vd.dtype, ks.dtype, vs.dtype) != _CACHE_DTYPES or len(shape) != 4
+            or not (kd.is_contiguous() and vd.is_contiguous() and ks.is_contiguous()
+                    and vs.is_contiguous())):
         raise _lib.NvkError("Fp4Cache must be contiguous uint8 [num_blocks, Hkv, block_size, D / 2] "
                             "and float16 [num_blocks, Hkv, D / 32, block_size]")
+    nb, hkv, bs, half = shape
     if ((half != 64 and half != 32) or bs % 16 or vd.shape != shape
-            or ks.shape != (nb, hkv, half // 16, bs) or vs.shape != ks.shape):
+            or not ks.shape == vs.shape == (nb, hkv, half // 16, bs)):
         raise _lib.NvkError("Fp4Cache shapes disagree, or head_dim is not 128 or 64, or block_size "
                             "not a multiple of 16")
     return nb, bs, hkv, 2 * half
 
 
+_CACHE_DTYPES = (torch.uint8, torch.uint8, torch.float16, torch.float16)
+
+
 def _device(k_cache, v_cache, *tensors):
     """The GPU that the caches and the tensors are on (they have to share one)."""
-    first = k_cache.data
-    dev = first.device
-    for t in (k_cache.scale, *v_cache, *tensors):
+    (kd, ks), (vd, vs) = k_cache, v_cache
+    dev = kd.device
+    if not (kd.is_cuda and dev == ks.device == vd.device == vs.device):
+        _lib.require_gpu(kd, ks, vd, vs)    # raises
+    for t in tensors:
         if t.device != dev:
-            _lib.require_gpu(first, t)    # raises
-    if not first.is_cuda:
-        _lib.require_gpu(first)           # raises
+            _lib.require_gpu(kd, t)         # raises
     return dev
 
 
@@ -108,9 +109,9 @@ def fp4_store(key: torch.Tensor, value: torch.Tensor, k_cache: Fp4Cache, v_cache
     dtype = _rows_dtype(key.dtype)
     N = key.shape[0]
     assert key.shape == value.shape == (N, hkv, d) and key.dtype == value.dtype
-    (ks, kh, k1), (vs, vh, v1) = key.stride(), value.stride()
-    assert k1 == 1 and v1 == 1
-    assert kh == d and vh == d
+    ks, *k_inner = key.stride()
+    vs, *v_inner = value.stride()
+    assert k_inner == v_inner == [d, 1]
     assert slot_mapping.numel() == N
     dev = _device(k_cache, v_cache, key, value, slot_mapping)
     slots = _lib.int32(slot_mapping)
