@@ -54,7 +54,7 @@ struct AttnArgs {
   int64_t out_stride_tok, out_stride_head;
   int32_t* desc;  // [batch][Hkv][max_tiles] x 2: first and last wave of the group, -1 if empty
   float* rec;     // [n_waves][2][rec_rows][HD + 4]: O, m, l
-  int rec_rows, n_waves;
+  int rec_rows, n_waves, wave_shift;  // n_waves = 2^wave_shift
 };
 
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
@@ -95,6 +95,13 @@ __device__ __forceinline__ int seq_units(const AttnArgs& a, int s) {
 __device__ int unit_prefix(const AttnArgs& a, int* s_cs, int* s_wsum) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int B = a.batch;
+  if (B <= 64) {  // every wave makes the same one for itself: no barrier
+    const int n = lane < B ? seq_units(a, lane) : 0;
+    const int x = nvk_wave_scan_add(n);
+    if (lane < B) s_cs[lane + 1] = x;
+    if (lane == 0) s_cs[0] = 0;
+    return __builtin_amdgcn_readlane(x, 63);
+  }
   const int per = (B + 255) / 256;
   const int b0 = tid * per;
   int local = 0;
@@ -117,22 +124,17 @@ __device__ int unit_prefix(const AttnArgs& a, int* s_cs, int* s_wsum) {
   return total;
 }
 
-// T chunks over P waves: the first T % P waves take one more than the others.
+// T chunks over n_waves waves, a power of two: wave w takes [w T / n, (w + 1) T / n), so that the
+// waves with one chunk more are spread over the CUs.  Fewer chunks than waves: one each.
 struct Split {
-  int P, per, rem;
-  __device__ __forceinline__ int begin(int w) const { return w * per + (w < rem ? w : rem); }
-  __device__ __forceinline__ int owner(int c) const {  // of chunk c
-    const int big = rem * (per + 1);
-    return c < big ? c / (per + 1) : rem + (c - big) / per;
+  int T, P, shift;
+  __device__ __forceinline__ int begin(int w) const {
+    return P == T ? w : (int)((int64_t)w * T >> shift);
+  }
+  __device__ __forceinline__ int owner(int c) const {  // of chunk c; exact: below 2^43, and 53 bits
+    return P == T ? c : (int)(((double)((int64_t)(c + 1) << shift) - 1.0) / (double)T);
   }
 };
-__device__ __forceinline__ Split split_of(int T, int n_waves) {
-  Split x;
-  x.P = T < n_waves ? T : n_waves;
-  x.per = x.P ? T / x.P : 0;
-  x.rem = T - x.P * x.per;
-  return x;
-}
 
 // 16 bytes per lane straight into LDS: lane l writes [dst + 16 l, +16).  From base + the lane's
 // offset, or from the lane's own address.
@@ -214,7 +216,8 @@ __global__ __launch_bounds__(64 * kWavesPerWG, 2) void fp4_attention_kernel(Attn
         *reinterpret_cast<int2*>(a.desc + 2 * (int64_t)e) = make_int2(-1, -1);
     }
   }
-  const Split sp = split_of(uniform(Hkv * S), a.n_waves);
+  const int T = uniform(Hkv * S);
+  const Split sp{T, T < a.n_waves ? T : a.n_waves, a.wave_shift};
   const int wave = uniform(tid >> 6);
   const int w = blockIdx.x * kWavesPerWG + wave;
   if (w >= sp.P) return;
@@ -230,7 +233,7 @@ __global__ __launch_bounds__(64 * kWavesPerWG, 2) void fp4_attention_kernel(Attn
     const int rr = c0 - Hkv * uniform(s_cs[s]);
     const int unit = uniform(rr / n);
     k = uniform(rr - unit * n);
-    kvh = uniform(unit / tiles);
+    kvh = tiles == 1 ? unit : uniform(unit / tiles);
     tile = uniform(unit - kvh * tiles);
   }
   bool started_here = k == 0;
@@ -259,33 +262,48 @@ __global__ __launch_bounds__(64 * kWavesPerWG, 2) void fp4_attention_kernel(Attn
   // Byte offsets of a chunk's (16-key blocks') first row of codes, and of the same row's scales.
   struct Where {
     uint64_t row[kBlk], scale[kBlk];
+    int in_page;  // ONEPAGE: the chunk's first key in its page
   };
-  auto locate = [&](const Seq& x, int ss, int hh, int kk) {
+  auto locate = [&](int keys, int ss, int hh, int kk) {
     Where p;
     const const_i32* bt = (const_i32*)(a.block_tables + (int64_t)ss * a.bt_stride);
 #pragma unroll
     for (int b = 0; b < kBlk; ++b) {
       int key = kk * kCK + 16 * b;
-      if (key >= x.keys) key = kk * kCK;  // a block past the keys: any block, nothing of it counts
+      if (key >= keys) key = kk * kCK;  // a block past the keys: any block, nothing of it counts
       const int logical = a.bs_shift >= 0 ? key >> a.bs_shift : key / a.block_size;
       int page = bt[logical];
       if (page < 0 || page >= a.num_blocks) page = 0;
-      const uint32_t off = (uint32_t)(key - logical * a.block_size);
+      const int off = key - logical * a.block_size;
       const uint64_t head = (uint64_t)(uint32_t)page * page_bytes + (uint64_t)(uint32_t)hh * head_bytes;
-      p.row[b] = head + off * RB;
-      p.scale[b] = (head >> 3) + off * 2;  // 2 bytes of scale per 16 of codes
+      p.row[b] = head + (uint32_t)off * RB;
+      p.scale[b] = (head >> 3) + (uint32_t)off * 2;  // 2 bytes of scale per 16 of codes
+      p.in_page = off;
     }
     return p;
+  };
+  // The next chunk of the same sequence and head: mostly further down its page.
+  auto locate_next = [&](Where p, int keys, int ss, int hh, int kk) {
+    if (ONEPAGE && p.in_page + kCK < a.block_size) {
+      p.row[0] += kCK * RB;
+      p.scale[0] += kCK * 2;
+      p.in_page += kCK;
+      return p;
+    }
+    return locate(keys, ss, hh, kk);
   };
   auto pick = [](const uint64_t* v, int i) {  // v[i] of a lane's block i
     if constexpr (kBlk == 1) return v[0];
     else return i & 2 ? (i & 1 ? v[3] : v[2]) : (i & 1 ? v[1] : v[0]);
   };
-  auto issue = [&](const Where& p, uint32_t buf, kvec (&kraw)[4]) {
+  auto issue_keys = [&](const Where& p, kvec (&kraw)[4]) {
     const uint8_t* kp = a.k_data + (kBlk == 1 ? p.row[0] : pick(p.row, r >> 2)) + k_off;
 #pragma unroll
     for (int b = 0; b < 4; ++b)
       kraw[b] = __builtin_nontemporal_load(reinterpret_cast<const kvec*>(kp + 4 * b * RB));
+  };
+  auto issue_rest = [&](const Where& p, uint32_t buf) {
+    lds_load(s_base + (kBlk == 1 ? p.scale[0] : pick(p.scale, s_key >> 4)), buf + kVBytes);
 #pragma unroll
     for (int j = 0; j < kVBytes / 1024; ++j) {
       if constexpr (kBlk == 1) {
@@ -295,7 +313,6 @@ __global__ __launch_bounds__(64 * kWavesPerWG, 2) void fp4_attention_kernel(Attn
         lds_load(a.v_data + pick(p.row, row >> 4) + ((row & 15) * RB + vbyte), buf + 1024 * j);
       }
     }
-    lds_load(s_base + (kBlk == 1 ? p.scale[0] : pick(p.scale, s_key >> 4)), buf + kVBytes);
   };
 
   // per-group state
@@ -328,23 +345,27 @@ __global__ __launch_bounds__(64 * kWavesPerWG, 2) void fp4_attention_kernel(Attn
   };
 
   kvec kraw[4];
-  issue(locate(sq, s, kvh, k), buf0, kraw);
+  Where at = locate(sq.keys, s, kvh, k);
+  issue_keys(at, kraw);
+  issue_rest(at, buf0);
   start_group();
   uint32_t cur = 0;
+  // the next group
+  int ns = s, nkvh = kvh, ntile = tile, nn = n, ntiles = tiles;
+  Seq nsq = sq;
 
   for (int c = c0;; ++c) {
-    // ---- the next chunk's position
+    // ---- the next chunk: its values and scales go out now, its keys once this one's are used
     const bool last = c + 1 == c1;
     const bool group_end = k == n - 1;
-    int ns = s, nkvh = kvh, ntile = tile, nk = k + 1, nn = n, ntiles = tiles;
-    Seq nsq = sq;
-    if (group_end) {
-      nk = 0;
-      if (++ntile == tiles) {
-        ntile = 0;
-        if (++nkvh == Hkv) {
-          nkvh = 0;
-          if (!last) {
+    if (!last) {
+      if (!group_end) {
+        at = locate_next(at, sq.keys, s, kvh, k + 1);
+      } else {
+        if (++ntile == tiles) {
+          ntile = 0;
+          if (++nkvh == Hkv) {
+            nkvh = 0;
             int b = s + 1;
             while (s_cs[b + 1] == s_cs[b]) ++b;  // a next chunk exists
             ns = uniform(b);
@@ -353,15 +374,12 @@ __global__ __launch_bounds__(64 * kWavesPerWG, 2) void fp4_attention_kernel(Attn
             ntiles = uniform(tiles_of(a, nsq));
           }
         }
+        at = locate(nsq.keys, ns, nkvh, 0);
       }
     }
-    Where np;
-    if (!last) np = locate(nsq, ns, nkvh, nk);
-
     wait_all();
-    const uint32_t buf = buf0 + cur * kBuf;
-    kvec knext[4];
-    if (!last) issue(np, buf0 + (cur ^ 1) * kBuf, knext);
+    const uint32_t buf = buf0 + cur;
+    if (!last) issue_rest(at, buf0 + (kBuf - cur));
 
     // ---- scores of keys 16 g + 4 b + i, row r
     const int kbase = k * kCK;
@@ -411,6 +429,8 @@ __global__ __launch_bounds__(64 * kWavesPerWG, 2) void fp4_attention_kernel(Attn
             sc[b][e] = fmaf(t[b][e], (float)ks[b >> 1][4 * (b & 1) + e], sc[b][e]);
       }
     }
+
+    if (!last) issue_keys(at, kraw);
 
     // ---- mask, running maximum, probabilities
     const bool full = kbase + kCK - 1 <= full_limit;
@@ -530,19 +550,17 @@ __global__ __launch_bounds__(64 * kWavesPerWG, 2) void fp4_attention_kernel(Attn
       if (last) return;
       s = ns;
       sq = nsq;
-      kvh = uniform(nkvh);
-      tile = uniform(ntile);
+      kvh = nkvh;
+      tile = ntile;
       n = nn;
       tiles = ntiles;
       k = 0;
       started_here = true;
       start_group();
     } else {
-      k = uniform(nk);
+      ++k;
     }
-#pragma unroll
-    for (int b = 0; b < 4; ++b) kraw[b] = knext[b];
-    cur ^= 1;
+    cur = kBuf - cur;
   }
 }
 
@@ -560,11 +578,16 @@ __global__ __launch_bounds__(64 * W) void fp4_merge_kernel(AttnArgs a) {
   const int kvh = blockIdx.x / pairs / a.max_tiles;
   const int s = blockIdx.y;
   const int lane = threadIdx.x & 63, v = uniform(threadIdx.x >> 6);
-  const Seq sq = seq_of(a, s);
-  const int rows = min(sq.queries * a.G - tile * kR, a.rec_rows);  // of this tile
-  if (2 * pair >= rows) return;
   const int64_t e = ((int64_t)s * a.num_kv_heads + kvh) * a.max_tiles + tile;
-  const int2 desc = *reinterpret_cast<const int2*>(a.desc + 2 * e);
+  int2 desc = *reinterpret_cast<const int2*>(a.desc + 2 * e);
+  int row0 = s * a.n_query, queries = a.n_query;
+  if (a.cu_q) {
+    const Seq sq = seq_of(a, s);
+    row0 = sq.row0;
+    queries = sq.queries;
+  }
+  const int rows = min(queries * a.G - tile * kR, a.rec_rows);  // of this tile
+  if (2 * pair >= rows) return;
   const int p1 = desc.x, p2 = desc.y;
   if (p1 >= 0 && p1 == p2) return;  // finished by one wave
   const int half = lane / kLanes, d0 = 4 * (lane % kLanes);
@@ -634,13 +657,13 @@ __global__ __launch_bounds__(64 * W) void fp4_merge_kernel(AttnArgs a) {
   nvk_u32x2 wv;
   wv.x = E::pack2(O[0] * inv, O[1] * inv);
   wv.y = E::pack2(O[2] * inv, O[3] * inv);
-  *reinterpret_cast<nvk_u32x2*>(a.out + (int64_t)(sq.row0 + tok) * a.out_stride_tok +
+  *reinterpret_cast<nvk_u32x2*>(a.out + (int64_t)(row0 + tok) * a.out_stride_tok +
                                 (int64_t)head * a.out_stride_head + d0) = wv;
 }
 
 // Sizes that follow from a call's static bounds.
 struct Plan {
-  int max_tiles, rec_rows, n_waves;
+  int max_tiles, rec_rows, n_waves, wave_shift;
   size_t desc_bytes, bytes;
 };
 bool plan_of(int batch, int max_queries, int num_q_heads, int num_kv_heads, int head_dim,
@@ -661,14 +684,20 @@ bool plan_of(int batch, int max_queries, int num_q_heads, int num_kv_heads, int 
   p.max_tiles = (int)tiles;
   p.rec_rows = (int)(rows < kR ? rows : kR);
   const int64_t units = tiles * chunks * batch * num_kv_heads;
-  int64_t wgs = (units + kWavesPerWG - 1) / kWavesPerWG;
-  if (wgs > kMaxWGs) wgs = kMaxWGs;
-  p.n_waves = (int)wgs * kWavesPerWG;
+  p.wave_shift = 2;  // a workgroup's
+  while ((1 << p.wave_shift) < units && (1 << p.wave_shift) < kMaxWGs * kWavesPerWG) ++p.wave_shift;
+  p.n_waves = 1 << p.wave_shift;
   p.desc_bytes = ((size_t)batch * num_kv_heads * tiles * 8 + 255) / 256 * 256;
   p.bytes = p.desc_bytes + (size_t)p.n_waves * 2 * p.rec_rows * (head_dim + 4) * sizeof(float);
   return true;
 }
 
+#ifndef NVK_M16
+#define NVK_M16 32
+#endif
+#ifndef NVK_M4
+#define NVK_M4 4
+#endif
 template <int HD, bool F16>
 int launch(const AttnArgs& a, hipStream_t s) {
   const dim3 grid(a.n_waves / kWavesPerWG), block(64 * kWavesPerWG);
@@ -683,9 +712,12 @@ int launch(const AttnArgs& a, hipStream_t s) {
   const int st = nvk_launch_status();
   if (st != NVK_OK) return st;
   const dim3 mgrid(a.num_kv_heads * a.max_tiles * ((a.rec_rows + 1) / 2), a.batch);
-  // 32 waves and more per group: its parts are folded by 16 waves
-  if (a.n_waves >= 32 * (int64_t)a.batch * a.num_kv_heads * a.max_tiles)
+  // by the parts a group may have: 8 of them are one round trip of a wave
+  const int64_t parts = a.n_waves / ((int64_t)a.batch * a.num_kv_heads * a.max_tiles);
+  if (parts >= NVK_M16)
     hipLaunchKernelGGL((fp4_merge_kernel<HD, F16, 16>), mgrid, dim3(64 * 16), 0, s, a);
+  else if (parts >= NVK_M4)
+    hipLaunchKernelGGL((fp4_merge_kernel<HD, F16, 4>), mgrid, dim3(64 * 4), 0, s, a);
   else
     hipLaunchKernelGGL((fp4_merge_kernel<HD, F16, 1>), mgrid, dim3(64), 0, s, a);
   return nvk_launch_status();
@@ -884,6 +916,7 @@ extern "C" int nvk_fp4_attention(const void* q, int64_t q_stride_tok, int64_t q_
   a.rec = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.desc_bytes);
   a.rec_rows = p.rec_rows;
   a.n_waves = p.n_waves;
+  a.wave_shift = p.wave_shift;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const bool f16 = dtype == NVK_DTYPE_F16;
   if (pages) return launch_pages(a, pp, num_q_heads, scale, f16, workspace, s);
