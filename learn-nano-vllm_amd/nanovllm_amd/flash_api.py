@@ -249,11 +249,14 @@ def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, rotary_cos=None
     Without block_table the caches are [B, S, Hkv, D]: sequence b is then one
     page of S slots.  The caches may be ``Fp4Cache``.
     """
-    _unsupported(k=(k, None), v=(v, None), rotary_cos=(rotary_cos, None),
-                 rotary_sin=(rotary_sin, None), cache_batch_idx=(cache_batch_idx, None),
-                 cache_leftpad=(cache_leftpad, None), window_size=(tuple(window_size), (-1, -1)),
-                 softcap=(softcap, 0.0), alibi_slopes=(alibi_slopes, None),
-                 return_softmax_lse=(return_softmax_lse, False))
+    if not (k is v is rotary_cos is rotary_sin is cache_batch_idx is cache_leftpad is alibi_slopes
+            is None and window_size == (-1, -1) and softcap == 0.0 and return_softmax_lse is False):
+        _unsupported(k=(k, None), v=(v, None), rotary_cos=(rotary_cos, None),
+                     rotary_sin=(rotary_sin, None), cache_batch_idx=(cache_batch_idx, None),
+                     cache_leftpad=(cache_leftpad, None),
+                     window_size=(tuple(window_size), (-1, -1)), softcap=(softcap, 0.0),
+                     alibi_slopes=(alibi_slopes, None),
+                     return_softmax_lse=(return_softmax_lse, False))
     if q.dim() != 4:
         raise _lib.NvkError("q must be [batch, seqlen_q, heads, head_dim]")
     b, sq, hq, d = q.shape

@@ -76,13 +76,13 @@ _CACHE_DTYPES = (torch.uint8, torch.uint8, torch.float16, torch.float16)
 def _device(k_cache, v_cache, *tensors):
     """The GPU that the caches and the tensors are on (they have to share one)."""
     (kd, ks), (vd, vs) = k_cache, v_cache
-    dev = kd.device
-    if not (kd.is_cuda and dev == ks.device == vd.device == vs.device):
+    gpu = kd.get_device()
+    if not 0 <= gpu == ks.get_device() == vd.get_device() == vs.get_device():
         _lib.require_gpu(kd, ks, vd, vs)    # raises
     for t in tensors:
-        if t.device != dev:
+        if t.get_device() != gpu:
             _lib.require_gpu(kd, t)         # raises
-    return dev
+    return kd.device
 
 
 _ROWS = {torch.bfloat16: _lib.NVK_DTYPE_BF16, torch.float16: _lib.NVK_DTYPE_F16}
@@ -158,20 +158,22 @@ def fp4_attention(q: torch.Tensor, k_cache: Fp4Cache, v_cache: Fp4Cache, seqlens
     nb, bs, hkv, d = _check_caches(k_cache, v_cache)
     dtype = _rows_dtype(q.dtype)
     shape, strides = q.shape, q.stride()
-    if len(shape) == 4 and cu_seqlens_q is None and out is None and shape[1] == max_seqlen_q:
-        if shape[1] != 1 and strides[0] != shape[1] * strides[1]:
+    if len(shape) == 3:
+        tq, hq, dq = shape
+        row, head, last = strides
+    elif len(shape) == 4 and cu_seqlens_q is None and out is None and shape[1] == max_seqlen_q:
+        b, n, hq, dq = shape
+        tq = b * n
+        seq, row, head, last = strides
+        if n == 1:
+            row = seq
+        elif seq != n * row:
             q = q.contiguous()
-            strides = q.stride()
-        tq, (row, head, last) = shape[0] * shape[1], strides[1:]
-        if shape[1] == 1:
-            row = strides[0]
-    elif len(shape) == 3:
-        tq, (row, head, last) = shape[0], strides
+            row, head, last = q.stride()[1:]
     else:
         raise _lib.NvkError("q must be [tokens, heads, head_dim]")
-    if last != 1 or shape[-1] != d:
+    if last != 1 or dq != d:
         raise _lib.NvkError("q must have unit last stride and the caches' head_dim")
-    hq = shape[-2]
     lens, bt = _lib.int32(seqlens_k), _lib.int32(block_table)
     cu_q = None if cu_seqlens_q is None else _lib.int32(cu_seqlens_q)
     batch = lens.numel()
@@ -181,19 +183,19 @@ def fp4_attention(q: torch.Tensor, k_cache: Fp4Cache, v_cache: Fp4Cache, seqlens
         batch -= 1
     elif batch * max_seqlen_q != tq:
         raise _lib.NvkError("q and cache_seqlens disagree on the batch size")
-    if bt.dim() != 2 or bt.shape[0] != batch:
+    if bt.dim() != 2 or len(bt) != batch:
         raise _lib.NvkError("block_table must be [batch, max_blocks]")
-    dev = _device(k_cache, v_cache, q, lens, bt, *(() if cu_q is None else (cu_q,)))
+    dev = _device(k_cache, v_cache, q, lens, bt, lens if cu_q is None else cu_q)
     if out is None:
-        out = torch.empty_like(q) if q.is_contiguous() else torch.empty(shape, dtype=q.dtype,
-                                                                        device=dev)
         out_row, out_head = hq * d, d
+        out = torch.empty_like(q) if (row == out_row or tq < 2) and head == d else \
+            torch.empty(shape, dtype=q.dtype, device=dev)
     else:
         if out.shape != shape or out.dtype != q.dtype or out.device != dev or out.stride(-1) != 1:
             raise _lib.NvkError("out must be like q, with unit last stride")
         out_row, out_head = out.stride()[:2]
     scale = d ** -0.5 if softmax_scale is None else float(softmax_scale)
-    mq, mk, width = int(max_seqlen_q), int(max_seqlen_k or 0), bt.shape[1]
+    mq, mk, width = int(max_seqlen_q), int(max_seqlen_k or 0), bt.size(1)
     ws_bytes = _workspace_bytes(batch, mq, mk, hq, hkv, d, bs, width)
     with _lib.on_device(dev):
         stream = _lib.stream_ptr(dev)
@@ -201,7 +203,7 @@ def fp4_attention(q: torch.Tensor, k_cache: Fp4Cache, v_cache: Fp4Cache, seqlens
         code = _lib.load().nvk_fp4_attention(
             q.data_ptr(), row, head, tq, k_cache.data.data_ptr(), k_cache.scale.data_ptr(),
             v_cache.data.data_ptr(), v_cache.scale.data_ptr(), _lib.ptr(cu_q), lens.data_ptr(),
-            batch, mq, mk, bt.data_ptr(), bt.stride(0), width, bs, nb, hq, hkv, d, scale,
+            batch, mq, mk, bt.data_ptr(), width, width, bs, nb, hq, hkv, d, scale,
             out.data_ptr(), out_row, out_head, _lib.ptr(ws), ws_bytes, dtype, stream)
     if code:
         _lib.check(code)
