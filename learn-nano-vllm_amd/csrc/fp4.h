@@ -59,8 +59,11 @@ struct Fp4Expand {
   const uint16_t *k_scale, *v_scale;
   const int32_t* block_tables;
   int64_t bt_stride;
-  const int32_t* cu_k;
-  int batch, pages_per_seq, max_blocks, block_size, num_blocks, num_kv_heads;
+  const int32_t* cu_k;          // prefix sums of the keys; or, where lens is given:
+  const int32_t* lens;          // the keys of every sequence of the batch, this part's from `first` on,
+  int first, total_batch, n_query;
+  int32_t *cu_q_out, *cu_k_out;  // whose prefix sums are written here (null: they are already)
+  int batch, pages_per_seq, max_blocks, block_size, bs_shift, num_blocks, num_kv_heads;
   uint16_t *k_pages, *v_pages;  // [batch * pages_per_seq][kFp4Page][num_kv_heads][128]
   int32_t* tables;              // [batch][pages_per_seq]: the pages' numbers
   bool f16;                     // of an f16 model

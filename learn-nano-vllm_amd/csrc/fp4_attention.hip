@@ -185,13 +185,15 @@ struct KeyVec<64> {
 };
 
 // ONEPAGE: pages of a multiple of 64 keys, so that a chunk lies in one; else of a multiple of 16.
-// FEW: steps of at most 16 / NG rows per kv head (NG = D / 32 groups), e.g. the decode of up to 4
-// heads of 128.  16 columns are then a row's NG groups: column (row, group) holds the query in
-// that group's dimensions and zeros elsewhere, so that the MFMAs of all steps add up to a group's
-// own sum.  One product with the scale per score, not NG, and NG lanes add up; and a lane needs
-// P vs of its own group only, whose dimensions alone are kept of its output.
-template <int HD, bool F16, bool ONEPAGE, bool FEW>
-__global__ __launch_bounds__(64 * kWavesPerWG, 2) void fp4_attention_kernel(AttnArgs a) {
+// NC: columns of the 16 that a row takes, for steps of at most 16 / NC rows per kv head (NC = 4: the
+// decode of up to 4 heads of 128).  Column (row, c) holds the query in the dimensions of NG / NC of
+// the NG = D / 32 groups and zeros elsewhere, so the MFMAs of other columns' groups add nothing to it.
+// A score is then NG / NC products with scales in each of NC lanes, which add up, instead of NG in
+// one; and a lane needs P vs for its own groups only, whose dimensions alone are kept of its output.
+// W waves per workgroup.  WHOLE: a workgroup owns one group, its waves an equal part of the chunks
+// each; they join their states in LDS, and nothing is left to a second kernel.
+template <int HD, bool F16, bool ONEPAGE, int NC, int W = kWavesPerWG, bool WHOLE = false>
+__global__ __launch_bounds__(64 * W, W == kWavesPerWG ? 2 : 1) void fp4_attention_kernel(AttnArgs a) {
   using E = NvkElt<F16>;
   typedef typename E::vec8 vec8;
   typedef typename KeyVec<HD>::type kvec;
@@ -201,37 +203,53 @@ __global__ __launch_bounds__(64 * kWavesPerWG, 2) void fp4_attention_kernel(Attn
   constexpr int kBuf = kVBytes + 1024;     // and its scales (D = 64 uses half of the 1024)
   constexpr int kBlk = ONEPAGE ? 1 : 4;    // pages looked up per chunk
   constexpr int kRec = HD + 4;
-  constexpr int NS = FEW ? 1 : NG;         // groups whose scales a lane needs
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[kWavesPerWG * kBuf];
-  __shared__ int s_cs[kMaxBatch + 1];
+  constexpr int NS = NG / NC;              // groups of a column
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[W * kBuf];
+  __shared__ int s_cs[WHOLE ? 1 : kMaxBatch + 1];
   __shared__ int s_wsum[kWavesPerWG];
   const int tid = threadIdx.x, lane = tid & 63;
   const int r = lane & 15, g = lane >> 4;
   const int Hkv = a.num_kv_heads;
 
-  const int S = unit_prefix(a, s_cs, s_wsum);
-  if (blockIdx.x == 0) {  // groups that no wave visits
-    const int per = Hkv * a.max_tiles;
-    for (int e = tid; e < a.batch * per; e += 256) {
-      const int b = e / per;
-      if (s_cs[b + 1] == s_cs[b])
-        *reinterpret_cast<int2*>(a.desc + 2 * (int64_t)e) = make_int2(-1, -1);
-    }
-  }
-  const int T = uniform(Hkv * S);
-  const Split sp{T, T < a.n_waves ? T : a.n_waves, a.wave_shift};
   const int wave = uniform(tid >> 6);
-  const int w = blockIdx.x * kWavesPerWG + wave;
-  if (w >= sp.P) return;
-  const int c0 = sp.begin(w), c1 = sp.begin(w + 1);
-  if (c0 >= c1) return;
-
+  int T = 0, w = 0, c0, c1;
   // position: sequence s, kv head, tile, chunk k of n
-  int s = nvk_last_le(s_cs, a.batch, Hkv, c0, lane);
-  Seq sq = seq_of(a, s);
-  int n = uniform(chunks_of(sq)), tiles = uniform(tiles_of(a, sq));
-  int kvh, tile, k;
-  {
+  int s, n, tiles, kvh, tile, k;
+  Seq sq;
+  if constexpr (WHOLE) {
+    kvh = blockIdx.x;
+    s = blockIdx.y;
+    tile = 0;
+    sq = seq_of(a, s);
+    n = uniform(chunks_of(sq));
+    tiles = 1;
+    if (sq.queries <= 0) return;
+    c0 = n * wave / W;
+    c1 = n * (wave + 1) / W;
+    k = c0;
+  } else {
+    const int S = unit_prefix(a, s_cs, s_wsum);
+    if (blockIdx.x == 0) {  // groups that no wave visits
+      const int per = Hkv * a.max_tiles;
+      for (int e = tid; e < a.batch * per; e += 256) {
+        const int b = e / per;
+        if (s_cs[b + 1] == s_cs[b])
+          *reinterpret_cast<int2*>(a.desc + 2 * (int64_t)e) = make_int2(-1, -1);
+      }
+    }
+    T = uniform(Hkv * S);
+    w = blockIdx.x * W + wave;
+  }
+  const Split sp{T, T < a.n_waves ? T : a.n_waves, a.wave_shift};
+  if constexpr (!WHOLE) {
+    if (w >= sp.P) return;
+    c0 = sp.begin(w);
+    c1 = sp.begin(w + 1);
+    if (c0 >= c1) return;
+    s = nvk_last_le(s_cs, a.batch, Hkv, c0, lane);
+    sq = seq_of(a, s);
+    n = uniform(chunks_of(sq));
+    tiles = uniform(tiles_of(a, sq));
     const int rr = c0 - Hkv * uniform(s_cs[s]);
     const int unit = uniform(rr / n);
     k = uniform(rr - unit * n);
@@ -323,7 +341,7 @@ __global__ __launch_bounds__(64 * kWavesPerWG, 2) void fp4_attention_kernel(Attn
   float m_run = -INFINITY, l_part[2] = {0.f, 0.f};
   int tok = 0, head = 0, row_limit = 0, full_limit = 0;
   bool row_valid = false;
-  const int row = FEW ? r / NG : r, grp = r & (NG - 1);  // this column's (FEW: and its group)
+  const int row = r / NC, g0 = r % NC * NS;  // this column's row, and the first of its groups
   auto start_group = [&]() {
     const int rr = tile * kR + row;
     tok = a.G == 1 ? rr : (int)__umulhi((uint32_t)rr, a.g_inverse);
@@ -337,7 +355,7 @@ __global__ __launch_bounds__(64 * kWavesPerWG, 2) void fp4_attention_kernel(Attn
 #pragma unroll
     for (int i = 0; i < NG; ++i) {
       nvk_u32x4 v = {0u, 0u, 0u, 0u};
-      if (row_valid && (!FEW || i == grp)) v = *reinterpret_cast<const nvk_u32x4*>(qp + 32 * i);
+      if (row_valid && (NC == 1 || i / NS * NS == g0)) v = *reinterpret_cast<const nvk_u32x4*>(qp + 32 * i);
       qf[i] = __builtin_bit_cast(vec8, v);
     }
 #pragma unroll
@@ -346,19 +364,35 @@ __global__ __launch_bounds__(64 * kWavesPerWG, 2) void fp4_attention_kernel(Attn
     l_part[0] = l_part[1] = 0.f;
   };
 
+  // the d blocks that are kept of this lane's column, those of its groups; d0: dimension of o[0][0]
+  constexpr int kKeep = 2 * NS;
+  const int d0 = 32 * g0 + 4 * g;
+  auto kept = [&](nvk_f32x4 (&o)[kKeep]) {
+#pragma unroll
+    for (int j = 0; j < kKeep; ++j) {
+      o[j] = acc[j];
+#pragma unroll
+      for (int i = 1; i < NC; ++i)
+        if (g0 == i * NS) o[j] = acc[i * kKeep + j];
+    }
+  };
+
   kvec kraw[4];
-  Where at = locate(sq.keys, s, kvh, k);
-  issue_keys(at, kraw);
-  issue_rest(at);
+  Where at;
+  if (!WHOLE || c0 < c1) {
+    at = locate(sq.keys, s, kvh, k);
+    issue_keys(at, kraw);
+    issue_rest(at);
+  }
   start_group();
   // the next group
   int ns = s, nkvh = kvh, ntile = tile, nn = n, ntiles = tiles;
   Seq nsq = sq;
 
-  for (int c = c0;; ++c) {
+  for (int c = c0; !WHOLE || c < c1; ++c) {
     // ---- the next chunk: its keys go out once this one's are used, its values and scales at the end
     const bool last = c + 1 == c1;
-    const bool group_end = k == n - 1;
+    const bool group_end = !WHOLE && k == n - 1;
     if (!last) {
       if (!group_end) {
         at = locate_next(at, sq.keys, s, kvh, k + 1);
@@ -382,53 +416,41 @@ __global__ __launch_bounds__(64 * kWavesPerWG, 2) void fp4_attention_kernel(Attn
 
     // ---- scores of keys 16 g + 4 b + i, row r
     const int kbase = k * kCK;
-    nvk_f32x4 sc[4] = {};
+    nvk_f32x4 sc[4];
     auto scales = [&](int tensor, int i) {  // of this lane's 16 keys
       return (const __attribute__((address_space(3))) nvk_f16x8*)(size_t)(
           buf + kVBytes + (uint32_t)(128 * (NG * tensor + i) + 32 * g));
     };
-    if constexpr (FEW) {
-      const auto* kp = scales(0, grp);
+#pragma unroll
+    for (int j = 0; j < NS; ++j) {
+      const auto* kp = scales(0, g0 + j);
       const nvk_f16x8 ks[2] = {kp[0], kp[1]};
+      nvk_f32x4 t[4] = {};
 #pragma unroll
-      for (int i = 0; i < NG; ++i)
+      for (int i = j; i < NG; i += NS)
 #pragma unroll
-        for (int b = 0; b < 4; ++b)
-          sc[b] = E::mfma16x16x32(fp4_unpack<F16>(kraw[b][i]), qf[i], sc[b]);
+        for (int b = 0; b < 4; ++b) t[b] = E::mfma16x16x32(fp4_unpack<F16>(kraw[b][i]), qf[i], t[b]);
 #pragma unroll
       for (int b = 0; b < 4; ++b)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          sc[b][e] = fmaf(sc[b][e], (float)ks[b >> 1][4 * (b & 1) + e], 0.f);
+          sc[b][e] = fmaf(t[b][e], (float)ks[b >> 1][4 * (b & 1) + e], j ? sc[b][e] : 0.f);
+    }
+    if constexpr (NC > 1) {
 #pragma unroll
       for (int b = 0; b < 4; ++b)
 #pragma unroll
         for (int e = 0; e < 4; ++e) sc[b][e] += nvk_dpp<NVK_DPP_QP_XOR1>(sc[b][e]);
-      if constexpr (NG == 4) {
-#pragma unroll
-        for (int b = 0; b < 4; ++b)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) sc[b][e] += nvk_dpp<NVK_DPP_QP_XOR2>(sc[b][e]);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < NG; ++i) {
-        const auto* kp = scales(0, i);
-        const nvk_f16x8 ks[2] = {kp[0], kp[1]};
-        nvk_f32x4 t[4];
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          const nvk_f32x4 z = {0.f, 0.f, 0.f, 0.f};
-          t[b] = E::mfma16x16x32(fp4_unpack<F16>(kraw[b][i]), qf[i], z);
-        }
-#pragma unroll
-        for (int b = 0; b < 4; ++b)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            sc[b][e] = fmaf(t[b][e], (float)ks[b >> 1][4 * (b & 1) + e], sc[b][e]);
-      }
     }
-
+    if constexpr (NC > 2) {
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sc[b][e] += nvk_dpp<NVK_DPP_QP_XOR2>(sc[b][e]);
+    }
+    // finished here, and not behind the next branch, where the lane exchanges would be moves of their own
+#pragma unroll
+    for (int b = 0; b < 4; ++b) asm volatile("" : "+v"(sc[b]));
     if (!last) issue_keys(at, kraw);
 
     // ---- mask, running maximum, probabilities
@@ -465,11 +487,11 @@ __global__ __launch_bounds__(64 * kWavesPerWG, 2) void fp4_attention_kernel(Attn
       }
 
     // ---- O^T += V^T (P vs)^T, one operand per group of dimensions
-    vec8h pf[2];
+    vec8h pf[NS][2];
 #pragma unroll
     for (int i = 0; i < NG; ++i) {
       if (i < NS) {
-        const auto* vp = scales(1, FEW ? grp : i);
+        const auto* vp = scales(1, g0 + i);
         nvk_u32x4 vs[2] = {__builtin_bit_cast(nvk_u32x4, vp[0]), __builtin_bit_cast(nvk_u32x4, vp[1])};
         if (!full) {
           // a masked key's scale may be anything, what an earlier owner of the page left too
@@ -486,7 +508,7 @@ __global__ __launch_bounds__(64 * kWavesPerWG, 2) void fp4_attention_kernel(Attn
           for (int p = 0; p < 4; ++p)
             x[p] = times_scales(sc[2 * h + (p >> 1)][2 * (p & 1)], sc[2 * h + (p >> 1)][2 * (p & 1) + 1],
                                 vs[h][p]);
-          pf[h] = __builtin_bit_cast(vec8h, x);
+          pf[i][h] = __builtin_bit_cast(vec8h, x);
         }
       }
 #pragma unroll
@@ -495,8 +517,8 @@ __global__ __launch_bounds__(64 * kWavesPerWG, 2) void fp4_attention_kernel(Attn
         const i32x2 vc = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
             (__attribute__((address_space(3))) i32x2*)(size_t)(buf + tr_row + 16 * (i ^ sw) +
                                                                 8 * h));
-        acc[d] = NvkElt<true>::mfma16x16x32(fp4_unpack<true>((uint32_t)vc[0]), pf[0], acc[d]);
-        acc[d] = NvkElt<true>::mfma16x16x32(fp4_unpack<true>((uint32_t)vc[1]), pf[1], acc[d]);
+        acc[d] = NvkElt<true>::mfma16x16x32(fp4_unpack<true>((uint32_t)vc[0]), pf[i % NS][0], acc[d]);
+        acc[d] = NvkElt<true>::mfma16x16x32(fp4_unpack<true>((uint32_t)vc[1]), pf[i % NS][1], acc[d]);
       }
     }
 
@@ -506,21 +528,14 @@ __global__ __launch_bounds__(64 * kWavesPerWG, 2) void fp4_attention_kernel(Attn
     }
 
     // ---- the group's or the range's end
+    if (WHOLE) {
+      ++k;
+      continue;
+    }
     if (group_end || last) {
       const float l_tot = nvk_sum_xor32(sum_xor16(l_part[0] + l_part[1]));
-      // the d blocks that this lane's column is kept of: FEW: those of its group
-      constexpr int kKeep = FEW ? 2 : HD / 16;
       nvk_f32x4 o[kKeep];
-#pragma unroll
-      for (int j = 0; j < kKeep; ++j) {
-        o[j] = acc[j];
-        if constexpr (FEW) {
-#pragma unroll
-          for (int i = 1; i < NG; ++i)
-            if (grp == i) o[j] = acc[2 * i + j];
-        }
-      }
-      const int d0 = (FEW ? 32 * grp : 0) + 4 * g;  // dimension of o[0][0]
+      kept(o);
       if (group_end && started_here) {
         if (row_valid) {
           const float inv = l_tot == 0.f ? 0.f : 1.f / l_tot;
@@ -540,7 +555,7 @@ __global__ __launch_bounds__(64 * kWavesPerWG, 2) void fp4_attention_kernel(Attn
 #pragma unroll
         for (int j = 0; j < kKeep; ++j)
           *reinterpret_cast<nvk_f32x4*>(rec + d0 + 16 * j) = o[j];
-        if (g == 0 && (!FEW || grp == 0)) {
+        if (g == 0 && g0 == 0) {
           rec[HD] = m_run;
           rec[HD + 1] = l_tot;
         }
@@ -564,6 +579,51 @@ __global__ __launch_bounds__(64 * kWavesPerWG, 2) void fp4_attention_kernel(Attn
     } else {
       ++k;
     }
+  }
+
+  if constexpr (WHOLE) {
+    // Wave v's rows to LDS (the values' buffers, used up): O, m, l; then a thread sums 4 dimensions of
+    // a row over the waves.
+    static_assert(W * (kR / NC) * kRec * 4 <= W * kBuf, "the states fit the buffers");
+    float* st = reinterpret_cast<float*>(lds);
+    const float l_tot = nvk_sum_xor32(sum_xor16(l_part[0] + l_part[1]));
+    nvk_f32x4 o[kKeep];
+    kept(o);
+    wait_reads();
+    __syncthreads();
+    if (row_valid) {
+      float* rec = st + (wave * a.rec_rows + row) * kRec;
+#pragma unroll
+      for (int j = 0; j < kKeep; ++j) *reinterpret_cast<nvk_f32x4*>(rec + d0 + 16 * j) = o[j];
+      if (g == 0 && g0 == 0) {
+        rec[HD] = m_run;
+        rec[HD + 1] = l_tot;
+      }
+    }
+    __syncthreads();
+    const int mrow = tid / (HD / 4), d = 4 * (tid % (HD / 4));
+    if (mrow >= sq.queries * a.G || mrow >= a.rec_rows) return;
+    float M = -INFINITY;
+#pragma unroll
+    for (int v = 0; v < W; ++v) M = fmaxf(M, st[(v * a.rec_rows + mrow) * kRec + HD]);
+    const float mref = M == -INFINITY ? 0.f : M;
+    float L = 0.f;
+    nvk_f32x4 O = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int v = 0; v < W; ++v) {
+      const float* rec = st + (v * a.rec_rows + mrow) * kRec;
+      const float wt = nvk_fast_exp2(rec[HD] - mref);
+      L += rec[HD + 1] * wt;
+      O += wt * *reinterpret_cast<const nvk_f32x4*>(rec + d);
+    }
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    const int mt = a.G == 1 ? mrow : (int)__umulhi((uint32_t)mrow, a.g_inverse);
+    nvk_u32x2 wv;
+    wv.x = E::pack2(O[0] * inv, O[1] * inv);
+    wv.y = E::pack2(O[2] * inv, O[3] * inv);
+    *reinterpret_cast<nvk_u32x2*>(a.out + (int64_t)(sq.row0 + mt) * a.out_stride_tok +
+                                  (int64_t)(kvh * a.G + mrow - mt * a.G) * a.out_stride_head + d) =
+        wv;
   }
 }
 
@@ -695,31 +755,58 @@ bool plan_of(int batch, int max_queries, int num_q_heads, int num_kv_heads, int 
   return true;
 }
 
-#ifndef NVK_M16
-#define NVK_M16 32
-#endif
-#ifndef NVK_M4
-#define NVK_M4 4
-#endif
+// Whether a workgroup of 16 waves takes each group (WHOLE): one kernel less, for groups that are
+// few enough to have a CU each and short enough for one to stream.  Two chunks for a wave take a
+// CU 4 us longer than one, and more CUs then share a group's keys in less: unless there are groups for
+// many of them, or the second kernel, 3 us of the host's time, is what a call waits for.
+// Measured, graph replays, cut between waves / a workgroup each, 16/8 heads of 128:
+//   1 x 100 keys 7.8 / 6.0 us, 1 x 1000 8.7 / 7.7, 4 x 1024 9.4 / 8.5, 32 x U{100..1000} 14.3 / 10.1;
+//   1 x 1280 8.7 / 10.6, 1 x 2048 9.2 / 12.0, 4 x 2048 10.1 / 12.5 (called one by one: 16.3 / 13.6), 8 x
+//   2048 12.5 / 12.8, 12 x 2048 14.8 / 13.2, 32 x 2048 21.3 / 17.8;
+//   16 x U{100..3072} 16.1 / 17.4, 32 x U{100..3072} 18.9 / 19.1;
+//   33 x U{100..256} (264 groups) 9.2 / 10.3, 64 x U{100..300} 11.9 / 14.6.
+constexpr int kWholeWaves = 16;
+constexpr int64_t kWholeGroups = 256, kWholeKeys = 1024, kWholeMinGroups = 32;
+bool whole_groups(int rows, int head_dim, int64_t groups, int64_t max_keys) {
+  return rows <= kR / (head_dim / kFp4Group) && groups <= kWholeGroups &&
+         (max_keys <= kWholeKeys || (max_keys <= 2 * kWholeKeys && groups >= kWholeMinGroups));
+}
+
 template <int HD, bool F16>
 int launch(const AttnArgs& a, hipStream_t s) {
+  constexpr int NG = HD / kFp4Group;
   const dim3 grid(a.n_waves / kWavesPerWG), block(64 * kWavesPerWG);
-  const auto main = [&](auto one, auto few) {
-    hipLaunchKernelGGL((fp4_attention_kernel<HD, F16, decltype(one)::value, decltype(few)::value>),
-                       grid, block, 0, s, a);
-  };
   const std::true_type yes;
   const std::false_type no;
-  if (a.n_query * a.G <= kR / (HD / kFp4Group)) a.block_size % kCK ? main(no, yes) : main(yes, yes);
-  else a.block_size % kCK ? main(no, no) : main(yes, no);
+  if (whole_groups(a.n_query * a.G, HD, (int64_t)a.batch * a.num_kv_heads, a.cap)) {
+    const auto one_kernel = [&](auto one) {
+      hipLaunchKernelGGL((fp4_attention_kernel<HD, F16, decltype(one)::value, NG, kWholeWaves, true>),
+                         dim3(a.num_kv_heads, a.batch), dim3(64 * kWholeWaves), 0, s, a);
+    };
+    a.block_size % kCK ? one_kernel(no) : one_kernel(yes);
+    return nvk_launch_status();
+  }
+  const auto main = [&](auto nc) {
+    if (a.block_size % kCK)
+      hipLaunchKernelGGL((fp4_attention_kernel<HD, F16, false, decltype(nc)::value>), grid, block, 0,
+                         s, a);
+    else
+      hipLaunchKernelGGL((fp4_attention_kernel<HD, F16, true, decltype(nc)::value>), grid, block, 0, s,
+                         a);
+  };
+  const int rows = a.n_query * a.G;
+  if (rows <= kR / NG) main(std::integral_constant<int, NG>{});
+  else if (rows <= kR / 2) main(std::integral_constant<int, 2>{});
+  else main(std::integral_constant<int, 1>{});
   const int st = nvk_launch_status();
   if (st != NVK_OK) return st;
   const dim3 mgrid(a.num_kv_heads * a.max_tiles * ((a.rec_rows + 1) / 2), a.batch);
-  // by the parts a group may have: 8 of them are one round trip of a wave
+  // By the parts that a group has on average, where it has any: a wave fetches 8 in a round trip.
+  // 64 x U{100..2048} keys, 16/8 heads (4 parts): 24.4 us with one wave per row pair, 23.1 with four.
   const int64_t parts = a.n_waves / ((int64_t)a.batch * a.num_kv_heads * a.max_tiles);
-  if (parts >= NVK_M16)
+  if (parts >= 32)
     hipLaunchKernelGGL((fp4_merge_kernel<HD, F16, 16>), mgrid, dim3(64 * 16), 0, s, a);
-  else if (parts >= NVK_M4)
+  else if (parts >= 4)
     hipLaunchKernelGGL((fp4_merge_kernel<HD, F16, 4>), mgrid, dim3(64 * 4), 0, s, a);
   else
     hipLaunchKernelGGL((fp4_merge_kernel<HD, F16, 1>), mgrid, dim3(64), 0, s, a);
@@ -777,15 +864,17 @@ int launch_pages(const AttnArgs& a, const PagePlan& p, int num_q_heads, float sc
                  void* workspace, hipStream_t s) {
   char* at = static_cast<char*>(workspace);
   const int32_t *cu_q = a.cu_q, *cu_k = a.keys;
-  if (!cu_q) {
-    int32_t* cu = reinterpret_cast<int32_t*>(at);
-    const int st = nvk_uniform_cu_seqlens(a.keys, a.batch, a.n_query, cu, cu + a.batch + 1, s);
-    if (st != NVK_OK) return st;
-    cu_q = cu;
-    cu_k = cu + a.batch + 1;
+  Fp4Expand e{};
+  if (!cu_q) {  // the same number of queries each: the first pass makes the prefix sums as well
+    e.lens = a.keys;
+    e.total_batch = a.batch;
+    e.n_query = a.n_query;
+    e.cu_q_out = reinterpret_cast<int32_t*>(at);
+    e.cu_k_out = e.cu_q_out + a.batch + 1;
+    cu_q = e.cu_q_out;
+    cu_k = e.cu_k_out;
   }
   at += p.cu_bytes;
-  Fp4Expand e{};
   e.tables = reinterpret_cast<int32_t*>(at);
   at += p.table_bytes;
   e.k_pages = reinterpret_cast<uint16_t*>(at);
@@ -800,6 +889,7 @@ int launch_pages(const AttnArgs& a, const PagePlan& p, int num_q_heads, float sc
   e.pages_per_seq = p.pages_per_seq;
   e.max_blocks = a.cap / a.block_size;
   e.block_size = a.block_size;
+  e.bs_shift = a.bs_shift;
   e.num_blocks = a.num_blocks;
   e.num_kv_heads = a.num_kv_heads;
   e.f16 = f16;
@@ -828,7 +918,9 @@ int launch_pages(const AttnArgs& a, const PagePlan& p, int num_q_heads, float sc
     e.block_tables = a.block_tables + b * a.bt_stride;
     e.cu_k = f.cu_k = cu_k + b;
     f.cu_q = cu_q + b;
+    e.first = b;
     int st = fp4_expand_launch(e, s);
+    e.cu_q_out = e.cu_k_out = nullptr;
     if (st == NVK_OK) st = fp4_prefill_launch(f, s);
     if (st != NVK_OK) return st;
   }

@@ -148,41 +148,61 @@ __global__ __launch_bounds__(256) void fp4_load_kernel(CacheArgs a, uint16_t* ke
   *reinterpret_cast<nvk_u32x4*>(value + t * value_stride + col) = v;
 }
 
-// Keys and values of each sequence's pages as f16 (see Fp4Expand).  grid = (64-token pieces of a
-// sequence, kv heads, sequences); 16 lanes a row, 16 rows a pass.
+// Prefix sums of a batch whose sequences all have a.n_query queries, by one workgroup.
+__device__ void uniform_prefix(const Fp4Expand& a) {
+  __shared__ int s_sum[256];
+  const int per = (a.total_batch + 255) / 256, b0 = threadIdx.x * per;
+  int local = 0;
+  for (int i = 0; i < per; ++i)
+    if (b0 + i < a.total_batch) local += a.lens[b0 + i];
+  s_sum[threadIdx.x] = local;
+  __syncthreads();
+  int run = 0;
+  for (int t = 0; t < (int)threadIdx.x; ++t) run += s_sum[t];
+  for (int i = 0; i < per; ++i) {
+    if (b0 + i >= a.total_batch) break;
+    a.cu_q_out[b0 + i] = (b0 + i) * a.n_query;
+    a.cu_k_out[b0 + i] = run;
+    run += a.lens[b0 + i];
+    if (b0 + i + 1 == a.total_batch) {
+      a.cu_q_out[a.total_batch] = a.total_batch * a.n_query;
+      a.cu_k_out[a.total_batch] = run;
+    }
+  }
+}
+
+// Keys and values of each sequence's pages as f16 (see Fp4Expand).  grid = (16-token pieces of a
+// sequence, sequences); 16 lanes a row.  A workgroup goes through its tokens' heads, HB at a time:
+// the length and the page are looked up once for all of them, and what it writes is 16 whole rows of
+// a page.  Bound by the stores: 32 sequences of U{612..1536} tokens and 8 heads, 31 MB read and 110
+// written, take 40 us (HB 1 to 4: 42; a workgroup per piece and head, 1, 2 or 4 rows per thread: 48).
 template <bool F16>
 __global__ __launch_bounds__(256) void fp4_expand_kernel(Fp4Expand a) {
-  constexpr int HD = 128, kPass = 4;
-  const int s = blockIdx.z, h = blockIdx.y;
-  if (blockIdx.x == 0 && h == 0)
+  constexpr int HD = 128, HB = 8;
+  const int s = blockIdx.y;
+  if (blockIdx.x == 0) {
     for (int i = threadIdx.x; i < a.pages_per_seq; i += 256)
       a.tables[(int64_t)s * a.pages_per_seq + i] = s * a.pages_per_seq + i;
-  int64_t keys = (int64_t)a.cu_k[s + 1] - a.cu_k[s];
+    if (a.cu_q_out && s == 0) uniform_prefix(a);
+  }
+  int64_t keys = a.lens ? a.lens[a.first + s] : (int64_t)a.cu_k[s + 1] - a.cu_k[s];
   if (keys > (int64_t)a.pages_per_seq * kFp4Page) keys = (int64_t)a.pages_per_seq * kFp4Page;
   if (keys > (int64_t)a.max_blocks * a.block_size) keys = (int64_t)a.max_blocks * a.block_size;
   const int u = threadIdx.x % 16;
-  const int p0 = blockIdx.x * 16 * kPass + threadIdx.x / 16;
-  const int32_t* bt = a.block_tables + s * a.bt_stride;
-  uint32_t kc[kPass], vc[kPass];
-  uint16_t ks[kPass], vs[kPass];
-#pragma unroll
-  for (int i = 0; i < kPass; ++i) {
-    const int p = p0 + 16 * i;
-    if (p >= keys) continue;
-    const int logical = p / a.block_size;
-    int page = bt[logical];
-    if (page < 0 || page >= a.num_blocks) page = 0;
-    const int off = p - logical * a.block_size;
-    const int64_t head = (int64_t)page * a.num_kv_heads + h;
-    const int64_t row = head * a.block_size + off;
-    const int64_t srow = head * 4 * a.block_size + off + (int64_t)(u / 4) * a.block_size;
-    kc[i] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(
-        a.k_data + row * (HD / 2) + 4 * fp4_place<HD, true>(u)));
-    vc[i] = __builtin_nontemporal_load(
-        reinterpret_cast<const uint32_t*>(a.v_data + row * (HD / 2) + 4 * u));
-    ks[i] = a.k_scale[srow];
-    vs[i] = a.v_scale[srow];
-  }
+  const int p = blockIdx.x * 16 + threadIdx.x / 16;
+  if (p >= keys) return;  // whole rows
+  const int logical = a.bs_shift >= 0 ? p >> a.bs_shift : p / a.block_size;
+  int page = a.block_tables[s * a.bt_stride + logical];
+  if (page < 0 || page >= a.num_blocks) page = 0;
+  const int off = p - logical * a.block_size;
+  const int64_t head0 = (int64_t)page * a.num_kv_heads;
+  const int64_t row0 = head0 * a.block_size + off;                          // of head 0
+  const int64_t srow0 = head0 * 4 * a.block_size + off + (int64_t)(u / 4) * a.block_size;
+  const uint8_t* kp = a.k_data + row0 * (HD / 2) + 4 * fp4_place<HD, true>(u);
+  const uint8_t* vp = a.v_data + row0 * (HD / 2) + 4 * u;
+  const int64_t out0 =
+      ((int64_t)s * a.pages_per_seq * kFp4Page + p) * a.num_kv_heads * HD + 8 * u;
+  const int64_t head_bytes = (int64_t)a.block_size * (HD / 2);
   auto f16_values = [](uint32_t code, float s) {
     const auto c = __builtin_bit_cast(nvk_u32x4, fp4_unpack<true>(code));
     nvk_u32x4 o;
@@ -198,25 +218,36 @@ __global__ __launch_bounds__(256) void fp4_expand_kernel(Fp4Expand a) {
     return o;
   };
   constexpr float kUnit = F16 ? 1.f : 1.f / (1 << kFp4KeyShift);
+  for (int h0 = 0; h0 < a.num_kv_heads; h0 += HB) {
+    uint32_t kc[HB], vc[HB];
+    uint16_t ks[HB], vs[HB];
 #pragma unroll
-  for (int i = 0; i < kPass; ++i) {
-    const int p = p0 + 16 * i;
-    if (p >= keys) continue;  // whole rows: the lanes of a row leave together
-    const float fk = (float)__builtin_bit_cast(_Float16, ks[i]) * kUnit;
-    float fv = (float)__builtin_bit_cast(_Float16, vs[i]) * kUnit;
-    // A value that is not finite would meet the zero probability of a query that does not see
-    // it, as NaN.  It becomes 0 here and the row's key NaN, whose score a mask replaces.
-    const bool lost = !__builtin_isfinite(fk) || !__builtin_isfinite(fv);
-    const bool row_lost =
-        (__builtin_amdgcn_ballot_w64(lost) >> (threadIdx.x & 48) & 0xffffu) != 0;
-    if (!__builtin_isfinite(fv)) fv = 0.f;
-    nvk_u32x4 k = f16_values(kc[i], fk);
-    const nvk_u32x4 v = f16_values(vc[i], fv);
-    if (row_lost) k = nvk_u32x4{0x7e007e00u, 0x7e007e00u, 0x7e007e00u, 0x7e007e00u};
-    const int64_t at =
-        (((int64_t)s * a.pages_per_seq * kFp4Page + p) * a.num_kv_heads + h) * HD + 8 * u;
-    *reinterpret_cast<nvk_u32x4*>(a.k_pages + at) = k;
-    *reinterpret_cast<nvk_u32x4*>(a.v_pages + at) = v;
+    for (int i = 0; i < HB; ++i) {
+      const int h = h0 + i;
+      if (h >= a.num_kv_heads) continue;
+      kc[i] = *reinterpret_cast<const uint32_t*>(kp + h * head_bytes);
+      vc[i] = *reinterpret_cast<const uint32_t*>(vp + h * head_bytes);
+      ks[i] = a.k_scale[srow0 + (int64_t)h * 4 * a.block_size];
+      vs[i] = a.v_scale[srow0 + (int64_t)h * 4 * a.block_size];
+    }
+#pragma unroll
+    for (int i = 0; i < HB; ++i) {
+      const int h = h0 + i;
+      if (h >= a.num_kv_heads) continue;
+      const float fk = (float)__builtin_bit_cast(_Float16, ks[i]) * kUnit;
+      float fv = (float)__builtin_bit_cast(_Float16, vs[i]) * kUnit;
+      // A value that is not finite would meet the zero probability of a query that does not see
+      // it, as NaN.  It becomes 0 here and the row's key NaN, whose score a mask replaces.
+      const bool lost = !__builtin_isfinite(fk) || !__builtin_isfinite(fv);
+      const bool row_lost =
+          (__builtin_amdgcn_ballot_w64(lost) >> (threadIdx.x & 48) & 0xffffu) != 0;
+      if (!__builtin_isfinite(fv)) fv = 0.f;
+      nvk_u32x4 k = f16_values(kc[i], fk);
+      const nvk_u32x4 v = f16_values(vc[i], fv);
+      if (row_lost) k = nvk_u32x4{0x7e007e00u, 0x7e007e00u, 0x7e007e00u, 0x7e007e00u};
+      *reinterpret_cast<nvk_u32x4*>(a.k_pages + out0 + h * HD) = k;
+      *reinterpret_cast<nvk_u32x4*>(a.v_pages + out0 + h * HD) = v;
+    }
   }
 }
 
@@ -293,7 +324,7 @@ struct LoadLaunch {
 }  // namespace
 
 int fp4_expand_launch(const Fp4Expand& p, hipStream_t stream) {
-  const dim3 grid(p.pages_per_seq * (kFp4Page / 64), p.num_kv_heads, p.batch);
+  const dim3 grid(p.pages_per_seq * (kFp4Page / 16), p.batch);
   if (p.f16)
     hipLaunchKernelGGL(fp4_expand_kernel<true>, grid, dim3(256), 0, stream, p);
   else
