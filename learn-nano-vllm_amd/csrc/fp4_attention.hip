@@ -628,18 +628,17 @@ __global__ __launch_bounds__(64 * W, W == kWavesPerWG ? 2 : 1) void fp4_attentio
 }
 
 // Merges the records of groups cut between waves and writes the rows of groups without a key.
-// grid = (Hkv * max_tiles * row pairs of a tile, batch), W waves: a workgroup owns two rows of a group
+// grid = (max_tiles * row pairs of a tile, Hkv, batch), W waves: a workgroup owns two rows of a group
 // (HD / 4 lanes each, HD 64: half of them idle), wave v folds parts p1 + v, p1 + v + W, ... and wave 0
 // joins the waves' states through LDS.
 template <int HD, bool F16, int W>
 __global__ __launch_bounds__(64 * W) void fp4_merge_kernel(AttnArgs a) {
   using E = NvkElt<F16>;
-  constexpr int kRec = HD + 4, kLanes = HD / 4, kBatch = 8;
+  constexpr int kRec = HD + 4, kLanes = HD / 4, kBatch = 4;
   const int pairs = (a.rec_rows + 1) / 2;
-  const int pair = blockIdx.x % pairs;
-  const int tile = blockIdx.x / pairs % a.max_tiles;
-  const int kvh = blockIdx.x / pairs / a.max_tiles;
-  const int s = blockIdx.y;
+  const int tile = a.max_tiles == 1 ? 0 : blockIdx.x / pairs;
+  const int pair = blockIdx.x - tile * pairs;
+  const int kvh = blockIdx.y, s = blockIdx.z;
   const int lane = threadIdx.x & 63, v = uniform(threadIdx.x >> 6);
   const int64_t e = ((int64_t)s * a.num_kv_heads + kvh) * a.max_tiles + tile;
   int2 desc = *reinterpret_cast<const int2*>(a.desc + 2 * e);
@@ -664,17 +663,23 @@ __global__ __launch_bounds__(64 * W) void fp4_merge_kernel(AttnArgs a) {
       nvk_f32x4 ov[kBatch];
 #pragma unroll
       for (int u = 0; u < kBatch; ++u) {
-        const int p = base + u * W;
-        mv[u] = -INFINITY;
-        lv[u] = 0.f;
-        ov[u] = nvk_f32x4{0.f, 0.f, 0.f, 0.f};
-        if (p <= p2) {
-          const float* rec =
-              a.rec + (((int64_t)p * 2 + (p == p1 ? 0 : 1)) * a.rec_rows + row) * kRec;
-          mv[u] = rec[HD];
-          lv[u] = rec[HD + 1];
-          ov[u] = *reinterpret_cast<const nvk_f32x4*>(rec + d0);
-        }
+        // past the last part: it is read again, and replaced (a branch around each load would wait
+        // for it there, one after the other)
+        const int p = min(base + u * W, p2);
+        const float* rec =
+            a.rec + (((int64_t)p * 2 + (p == p1 ? 0 : 1)) * a.rec_rows + row) * kRec;
+        const float2 ml = *reinterpret_cast<const float2*>(rec + HD);
+        mv[u] = ml.x;
+        lv[u] = ml.y;
+        ov[u] = *reinterpret_cast<const nvk_f32x4*>(rec + d0);
+      }
+#pragma unroll
+      for (int u = 1; u < kBatch; ++u) {
+        const bool part = base + u * W <= p2;
+        mv[u] = part ? mv[u] : -INFINITY;
+        lv[u] = part ? lv[u] : 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ov[u][i] = part ? ov[u][i] : 0.f;
       }
       float mb = M;
 #pragma unroll
@@ -740,7 +745,7 @@ bool plan_of(int batch, int max_queries, int num_q_heads, int num_kv_heads, int 
   const int64_t rows = (int64_t)max_queries * G;
   const int64_t chunks = ((int64_t)max_blocks * block_size + kCK - 1) / kCK;
   const int64_t tiles = (rows + kR - 1) / kR;
-  if (rows >= 1 << 27 || tiles * num_kv_heads * 8 > INT32_MAX || chunks > INT32_MAX / kCK ||
+  if (rows >= 1 << 27 || num_kv_heads > 65535 || chunks > INT32_MAX / kCK ||
       tiles * chunks > INT32_MAX / batch / num_kv_heads ||
       (int64_t)block_size * num_kv_heads * head_dim > INT32_MAX)
     return false;
@@ -800,11 +805,12 @@ int launch(const AttnArgs& a, hipStream_t s) {
   else main(std::integral_constant<int, 1>{});
   const int st = nvk_launch_status();
   if (st != NVK_OK) return st;
-  const dim3 mgrid(a.num_kv_heads * a.max_tiles * ((a.rec_rows + 1) / 2), a.batch);
-  // By the parts that a group has on average, where it has any: a wave fetches 8 in a round trip.
-  // 64 x U{100..2048} keys, 16/8 heads (4 parts): 24.4 us with one wave per row pair, 23.1 with four.
+  const dim3 mgrid(a.max_tiles * ((a.rec_rows + 1) / 2), a.num_kv_heads, a.batch);
+  // By the parts that a group has on average, where it has any: a wave fetches 4 in a round trip.
+  // 64 x U{100..2048} keys, 16/8 heads (4 parts): 24.4 us with one wave per row pair, 23.1 with four; 32
+  // x 6 over U{1024..8192} (8 parts): 42.7 with one, 42.1 with four or sixteen.
   const int64_t parts = a.n_waves / ((int64_t)a.batch * a.num_kv_heads * a.max_tiles);
-  if (parts >= 32)
+  if (parts >= 16)
     hipLaunchKernelGGL((fp4_merge_kernel<HD, F16, 16>), mgrid, dim3(64 * 16), 0, s, a);
   else if (parts >= 4)
     hipLaunchKernelGGL((fp4_merge_kernel<HD, F16, 4>), mgrid, dim3(64 * 4), 0, s, a);

@@ -172,82 +172,79 @@ __device__ void uniform_prefix(const Fp4Expand& a) {
 }
 
 // Keys and values of each sequence's pages as f16 (see Fp4Expand).  grid = (16-token pieces of a
-// sequence, sequences); 16 lanes a row.  A workgroup goes through its tokens' heads, HB at a time:
-// the length and the page are looked up once for all of them, and what it writes is 16 whole rows of
-// a page.  Bound by the stores: 32 sequences of U{612..1536} tokens and 8 heads, 31 MB read and 110
-// written, take 40 us (HB 1 to 4: 42; a workgroup per piece and head, 1, 2 or 4 rows per thread: 48).
+// sequence, sequences, pairs of heads); 16 lanes a row.  32 sequences of U{612..1536} tokens and 8 heads,
+// 31 MB read and 110 written: 39 us; with all heads of a piece in a workgroup 41, with one head 48, and
+// other mappings (a quad per row, 4 heads of a token per wave, loads a step ahead) 41 to 48.
 template <bool F16>
 __global__ __launch_bounds__(256) void fp4_expand_kernel(Fp4Expand a) {
-  constexpr int HD = 128, HB = 8;
-  const int s = blockIdx.y;
-  if (blockIdx.x == 0) {
+  constexpr int HD = 128, HB = 2;
+  const int s = blockIdx.y, h0 = HB * blockIdx.z;
+  if (blockIdx.x == 0 && h0 == 0) {
     for (int i = threadIdx.x; i < a.pages_per_seq; i += 256)
       a.tables[(int64_t)s * a.pages_per_seq + i] = s * a.pages_per_seq + i;
     if (a.cu_q_out && s == 0) uniform_prefix(a);
   }
+  // the page is looked up beside the length, not after it
+  const int u = threadIdx.x % 16;
+  const int p = blockIdx.x * 16 + threadIdx.x / 16;
+  const int logical = a.bs_shift >= 0 ? p >> a.bs_shift : p / a.block_size;
+  int page = a.block_tables[s * a.bt_stride + min(logical, a.max_blocks - 1)];
   int64_t keys = a.lens ? a.lens[a.first + s] : (int64_t)a.cu_k[s + 1] - a.cu_k[s];
   if (keys > (int64_t)a.pages_per_seq * kFp4Page) keys = (int64_t)a.pages_per_seq * kFp4Page;
   if (keys > (int64_t)a.max_blocks * a.block_size) keys = (int64_t)a.max_blocks * a.block_size;
-  const int u = threadIdx.x % 16;
-  const int p = blockIdx.x * 16 + threadIdx.x / 16;
   if (p >= keys) return;  // whole rows
-  const int logical = a.bs_shift >= 0 ? p >> a.bs_shift : p / a.block_size;
-  int page = a.block_tables[s * a.bt_stride + logical];
   if (page < 0 || page >= a.num_blocks) page = 0;
   const int off = p - logical * a.block_size;
   const int64_t head0 = (int64_t)page * a.num_kv_heads;
-  const int64_t row0 = head0 * a.block_size + off;                          // of head 0
-  const int64_t srow0 = head0 * 4 * a.block_size + off + (int64_t)(u / 4) * a.block_size;
-  const uint8_t* kp = a.k_data + row0 * (HD / 2) + 4 * fp4_place<HD, true>(u);
-  const uint8_t* vp = a.v_data + row0 * (HD / 2) + 4 * u;
-  const int64_t out0 =
-      ((int64_t)s * a.pages_per_seq * kFp4Page + p) * a.num_kv_heads * HD + 8 * u;
-  const int64_t head_bytes = (int64_t)a.block_size * (HD / 2);
-  auto f16_values = [](uint32_t code, float s) {
-    const auto c = __builtin_bit_cast(nvk_u32x4, fp4_unpack<true>(code));
+  uint32_t kc[HB], vc[HB];
+  uint16_t ks[HB], vs[HB];
+#pragma unroll
+  for (int i = 0; i < HB; ++i) {
+    const int64_t head = head0 + min(h0 + i, a.num_kv_heads - 1);
+    const int64_t row = head * a.block_size + off;
+    const int64_t srow = head * 4 * a.block_size + off + (int64_t)(u / 4) * a.block_size;
+    kc[i] = *reinterpret_cast<const uint32_t*>(a.k_data + row * (HD / 2) +
+                                               4 * fp4_place<HD, true>(u));
+    vc[i] = *reinterpret_cast<const uint32_t*>(a.v_data + row * (HD / 2) + 4 * u);
+    ks[i] = a.k_scale[srow];
+    vs[i] = a.v_scale[srow];
+  }
+  // products of f16 numbers (the codes exact, times 2^-kFp4KeyShift or 1), each rounded once
+  auto f16_values = [](uint32_t code, _Float16 s) {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    constexpr float kUnit = F16 ? 1.f : 1.f / (1 << kFp4KeyShift);
+    const h2 ss = {s, s}, top = {(_Float16)65504.f, (_Float16)65504.f};
+    h2 c[4] = {__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(code, kUnit, 0),
+               __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(code, kUnit, 1),
+               __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(code, kUnit, 2),
+               __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(code, kUnit, 3)};
     nvk_u32x4 o;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      float lo = NvkElt<true>::lo(c[i]) * s, hi = NvkElt<true>::hi(c[i]) * s;
-      if constexpr (F16) {  // fmin / fmax drop a NaN: it goes into the keys below
-        lo = fminf(fmaxf(lo, -65504.f), 65504.f);
-        hi = fminf(fmaxf(hi, -65504.f), 65504.f);
-      }
-      o[i] = NvkElt<true>::pack2(lo, hi);
+      c[i] *= ss;
+      // (min and max drop a NaN: it goes into the keys below)
+      if constexpr (F16) c[i] = __builtin_elementwise_max(__builtin_elementwise_min(c[i], top), -top);
+      o[i] = __builtin_bit_cast(uint32_t, c[i]);
     }
     return o;
   };
-  constexpr float kUnit = F16 ? 1.f : 1.f / (1 << kFp4KeyShift);
-  for (int h0 = 0; h0 < a.num_kv_heads; h0 += HB) {
-    uint32_t kc[HB], vc[HB];
-    uint16_t ks[HB], vs[HB];
 #pragma unroll
-    for (int i = 0; i < HB; ++i) {
-      const int h = h0 + i;
-      if (h >= a.num_kv_heads) continue;
-      kc[i] = *reinterpret_cast<const uint32_t*>(kp + h * head_bytes);
-      vc[i] = *reinterpret_cast<const uint32_t*>(vp + h * head_bytes);
-      ks[i] = a.k_scale[srow0 + (int64_t)h * 4 * a.block_size];
-      vs[i] = a.v_scale[srow0 + (int64_t)h * 4 * a.block_size];
-    }
-#pragma unroll
-    for (int i = 0; i < HB; ++i) {
-      const int h = h0 + i;
-      if (h >= a.num_kv_heads) continue;
-      const float fk = (float)__builtin_bit_cast(_Float16, ks[i]) * kUnit;
-      float fv = (float)__builtin_bit_cast(_Float16, vs[i]) * kUnit;
-      // A value that is not finite would meet the zero probability of a query that does not see
-      // it, as NaN.  It becomes 0 here and the row's key NaN, whose score a mask replaces.
-      const bool lost = !__builtin_isfinite(fk) || !__builtin_isfinite(fv);
-      const bool row_lost =
-          (__builtin_amdgcn_ballot_w64(lost) >> (threadIdx.x & 48) & 0xffffu) != 0;
-      if (!__builtin_isfinite(fv)) fv = 0.f;
-      nvk_u32x4 k = f16_values(kc[i], fk);
-      const nvk_u32x4 v = f16_values(vc[i], fv);
-      if (row_lost) k = nvk_u32x4{0x7e007e00u, 0x7e007e00u, 0x7e007e00u, 0x7e007e00u};
-      *reinterpret_cast<nvk_u32x4*>(a.k_pages + out0 + h * HD) = k;
-      *reinterpret_cast<nvk_u32x4*>(a.v_pages + out0 + h * HD) = v;
-    }
+  for (int i = 0; i < HB; ++i) {
+    const int h = h0 + i;
+    if (h >= a.num_kv_heads) continue;  // uniform
+    // A value that is not finite would meet the zero probability of a query that does not see
+    // it, as NaN.  It becomes 0 here and the row's key NaN, whose score a mask replaces.
+    const bool v_lost = (vs[i] & 0x7c00) == 0x7c00;
+    const bool lost = v_lost || (ks[i] & 0x7c00) == 0x7c00;
+    const bool row_lost = (__builtin_amdgcn_ballot_w64(lost) >> (threadIdx.x & 48) & 0xffffu) != 0;
+    nvk_u32x4 k = f16_values(kc[i], __builtin_bit_cast(_Float16, ks[i]));
+    const nvk_u32x4 v =
+        f16_values(vc[i], v_lost ? (_Float16)0.f : __builtin_bit_cast(_Float16, vs[i]));
+    if (row_lost) k = nvk_u32x4{0x7e007e00u, 0x7e007e00u, 0x7e007e00u, 0x7e007e00u};
+    const int64_t at =
+        (((int64_t)s * a.pages_per_seq * kFp4Page + p) * a.num_kv_heads + h) * HD + 8 * u;
+    *reinterpret_cast<nvk_u32x4*>(a.k_pages + at) = k;
+    *reinterpret_cast<nvk_u32x4*>(a.v_pages + at) = v;
   }
 }
 
@@ -324,7 +321,7 @@ struct LoadLaunch {
 }  // namespace
 
 int fp4_expand_launch(const Fp4Expand& p, hipStream_t stream) {
-  const dim3 grid(p.pages_per_seq * (kFp4Page / 16), p.batch);
+  const dim3 grid(p.pages_per_seq * (kFp4Page / 16), p.batch, (p.num_kv_heads + 1) / 2);
   if (p.f16)
     hipLaunchKernelGGL(fp4_expand_kernel<true>, grid, dim3(256), 0, stream, p);
   else
