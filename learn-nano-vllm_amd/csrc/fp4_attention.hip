@@ -28,7 +28,7 @@
 
 namespace {
 
-constexpr int kR = 16;                   // rows of a tile
+constexpr int kR = 16;                   // columns of an MFMA: rows (query x head) of a tile, or half of one
 constexpr int kCK = 64;                  // keys of a chunk
 constexpr int kWavesPerWG = 4;
 constexpr int kMaxWGs = 512;             // two workgroups per CU
@@ -48,7 +48,7 @@ struct AttnArgs {
   const int32_t* keys;   // cu_seqlens_k, or context lengths
   const int32_t* block_tables;
   int64_t bt_stride;
-  int batch, n_query, max_tiles, cap, block_size, num_blocks;
+  int batch, n_query, tile_rows, max_tiles, cap, block_size, num_blocks;
   int bs_shift;          // log2 of block_size, or -1
   int num_kv_heads, G;
   uint32_t g_inverse;    // ceil(2^32 / G): rows (below 2^27) / G as a high product (G > 1)
@@ -86,7 +86,7 @@ __device__ __forceinline__ Seq seq_of(const AttnArgs& a, int s) {
   return x;
 }
 __device__ __forceinline__ int tiles_of(const AttnArgs& a, const Seq& x) {
-  return (x.queries * a.G + kR - 1) / kR;
+  return (x.queries * a.G + a.tile_rows - 1) / a.tile_rows;
 }
 __device__ __forceinline__ int chunks_of(const Seq& x) { return (x.keys + kCK - 1) / kCK; }
 __device__ __forceinline__ int seq_units(const AttnArgs& a, int s) {
@@ -190,9 +190,11 @@ struct KeyVec<64> {
 // the NG = D / 32 groups and zeros elsewhere, so the MFMAs of other columns' groups add nothing to it.
 // A score is then NG / NC products with scales in each of NC lanes, which add up, instead of NG in
 // one; and a lane needs P vs for its own groups only, whose dimensions alone are kept of its output.
+// NT: 16-row blocks of a tile.  Two share what the wave loads and converts (see wide_tiles).
 // W waves per workgroup.  WHOLE: a workgroup owns one group, its waves an equal part of the chunks
 // each; they join their states in LDS, and nothing is left to a second kernel.
-template <int HD, bool F16, bool ONEPAGE, int NC, int W = kWavesPerWG, bool WHOLE = false>
+template <int HD, bool F16, bool ONEPAGE, int NC, int NT = 1, int W = kWavesPerWG,
+          bool WHOLE = false>
 __global__ __launch_bounds__(64 * W, W == kWavesPerWG ? 2 : 1) void fp4_attention_kernel(AttnArgs a) {
   using E = NvkElt<F16>;
   typedef typename E::vec8 vec8;
@@ -336,44 +338,48 @@ __global__ __launch_bounds__(64 * W, W == kWavesPerWG ? 2 : 1) void fp4_attentio
   };
 
   // per-group state
-  vec8 qf[NG];
-  nvk_f32x4 acc[HD / 16];
-  float m_run = -INFINITY, l_part[2] = {0.f, 0.f};
-  int tok = 0, head = 0, row_limit = 0, full_limit = 0;
-  bool row_valid = false;
+  vec8 qf[NT][NG];
+  nvk_f32x4 acc[NT][HD / 16];
+  float m_run[NT], l_part[NT][2];
+  int tok[NT], head[NT], row_limit[NT], full_limit = 0;
+  bool row_valid[NT];
   const int row = r / NC, g0 = r % NC * NS;  // this column's row, and the first of its groups
   auto start_group = [&]() {
-    const int rr = tile * kR + row;
-    tok = a.G == 1 ? rr : (int)__umulhi((uint32_t)rr, a.g_inverse);
-    head = kvh * a.G + rr - tok * a.G;
-    row_valid = tok < sq.queries;
-    const int diag = sq.raw_keys - sq.queries;
-    row_limit = row_valid ? min(sq.keys - 1, diag + tok) : -1;           // last visible key
-    full_limit = uniform(min(sq.keys - 1, diag + tile * kR / a.G));      // visible to every row
-    const uint16_t* qp = a.q + (int64_t)(sq.row0 + tok) * a.q_stride_tok +
-                         (int64_t)head * a.q_stride_head + 8 * g;
+    const int diag = sq.raw_keys - sq.queries, rr0 = tile * kR * NT;
+    full_limit = uniform(min(sq.keys - 1, diag + rr0 / a.G));            // visible to every row
 #pragma unroll
-    for (int i = 0; i < NG; ++i) {
-      nvk_u32x4 v = {0u, 0u, 0u, 0u};
-      if (row_valid && (NC == 1 || i / NS * NS == g0)) v = *reinterpret_cast<const nvk_u32x4*>(qp + 32 * i);
-      qf[i] = __builtin_bit_cast(vec8, v);
+    for (int t = 0; t < NT; ++t) {
+      const int rr = rr0 + kR * t + row;
+      tok[t] = a.G == 1 ? rr : (int)__umulhi((uint32_t)rr, a.g_inverse);
+      head[t] = kvh * a.G + rr - tok[t] * a.G;
+      row_valid[t] = tok[t] < sq.queries;
+      row_limit[t] = row_valid[t] ? min(sq.keys - 1, diag + tok[t]) : -1;  // last visible key
+      const uint16_t* qp = a.q + (int64_t)(sq.row0 + tok[t]) * a.q_stride_tok +
+                           (int64_t)head[t] * a.q_stride_head + 8 * g;
+#pragma unroll
+      for (int i = 0; i < NG; ++i) {
+        nvk_u32x4 v = {0u, 0u, 0u, 0u};
+        if (row_valid[t] && (NC == 1 || i / NS * NS == g0))
+          v = *reinterpret_cast<const nvk_u32x4*>(qp + 32 * i);
+        qf[t][i] = __builtin_bit_cast(vec8, v);
+      }
+#pragma unroll
+      for (int d = 0; d < HD / 16; ++d) acc[t][d] = nvk_f32x4{0.f, 0.f, 0.f, 0.f};
+      m_run[t] = -INFINITY;
+      l_part[t][0] = l_part[t][1] = 0.f;
     }
-#pragma unroll
-    for (int d = 0; d < HD / 16; ++d) acc[d] = nvk_f32x4{0.f, 0.f, 0.f, 0.f};
-    m_run = -INFINITY;
-    l_part[0] = l_part[1] = 0.f;
   };
 
   // the d blocks that are kept of this lane's column, those of its groups; d0: dimension of o[0][0]
   constexpr int kKeep = 2 * NS;
   const int d0 = 32 * g0 + 4 * g;
-  auto kept = [&](nvk_f32x4 (&o)[kKeep]) {
+  auto kept = [&](nvk_f32x4 (&o)[kKeep], int t) {
 #pragma unroll
     for (int j = 0; j < kKeep; ++j) {
-      o[j] = acc[j];
+      o[j] = acc[t][j];
 #pragma unroll
       for (int i = 1; i < NC; ++i)
-        if (g0 == i * NS) o[j] = acc[i * kKeep + j];
+        if (g0 == i * NS) o[j] = acc[t][i * kKeep + j];
     }
   };
 
@@ -416,7 +422,7 @@ __global__ __launch_bounds__(64 * W, W == kWavesPerWG ? 2 : 1) void fp4_attentio
 
     // ---- scores of keys 16 g + 4 b + i, row r
     const int kbase = k * kCK;
-    nvk_f32x4 sc[4];
+    nvk_f32x4 sc[NT][4];
     auto scales = [&](int tensor, int i) {  // of this lane's 16 keys
       return (const __attribute__((address_space(3))) nvk_f16x8*)(size_t)(
           buf + kVBytes + (uint32_t)(128 * (NG * tensor + i) + 32 * g));
@@ -425,90 +431,111 @@ __global__ __launch_bounds__(64 * W, W == kWavesPerWG ? 2 : 1) void fp4_attentio
     for (int j = 0; j < NS; ++j) {
       const auto* kp = scales(0, g0 + j);
       const nvk_f16x8 ks[2] = {kp[0], kp[1]};
-      nvk_f32x4 t[4] = {};
+      nvk_f32x4 x[NT][4] = {};
 #pragma unroll
       for (int i = j; i < NG; i += NS)
 #pragma unroll
-        for (int b = 0; b < 4; ++b) t[b] = E::mfma16x16x32(fp4_unpack<F16>(kraw[b][i]), qf[i], t[b]);
+        for (int b = 0; b < 4; ++b) {
+          const vec8 kf = fp4_unpack<F16>(kraw[b][i]);
 #pragma unroll
-      for (int b = 0; b < 4; ++b)
+          for (int t = 0; t < NT; ++t) x[t][b] = E::mfma16x16x32(kf, qf[t][i], x[t][b]);
+        }
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          sc[b][e] = fmaf(t[b][e], (float)ks[b >> 1][4 * (b & 1) + e], j ? sc[b][e] : 0.f);
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            sc[t][b][e] = fmaf(x[t][b][e], (float)ks[b >> 1][4 * (b & 1) + e], j ? sc[t][b][e] : 0.f);
+      if constexpr (NT > 1) __builtin_amdgcn_sched_barrier(0);  // a group's operands at a time
     }
+    static_assert(NC == 1 || NT == 1, "columns of a row within one block");
     if constexpr (NC > 1) {
 #pragma unroll
       for (int b = 0; b < 4; ++b)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sc[b][e] += nvk_dpp<NVK_DPP_QP_XOR1>(sc[b][e]);
+        for (int e = 0; e < 4; ++e) sc[0][b][e] += nvk_dpp<NVK_DPP_QP_XOR1>(sc[0][b][e]);
     }
     if constexpr (NC > 2) {
 #pragma unroll
       for (int b = 0; b < 4; ++b)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sc[b][e] += nvk_dpp<NVK_DPP_QP_XOR2>(sc[b][e]);
+        for (int e = 0; e < 4; ++e) sc[0][b][e] += nvk_dpp<NVK_DPP_QP_XOR2>(sc[0][b][e]);
     }
-    // finished here, and not behind the next branch, where the lane exchanges would be moves of their own
+    // finished here, and not behind the next branch: the lane exchanges would be moves of their own
+    // there, and the products of every group be kept until then
 #pragma unroll
-    for (int b = 0; b < 4; ++b) asm volatile("" : "+v"(sc[b]));
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int b = 0; b < 4; ++b) asm volatile("" : "+v"(sc[t][b]));
     if (!last) issue_keys(at, kraw);
 
     // ---- mask, running maximum, probabilities
     const bool full = kbase + kCK - 1 <= full_limit;
-    const int seen = row_limit - kbase - 16 * g + 1;  // of this lane's 16 keys, the first `seen`
-    if (!full) {
+    int seen[NT];  // of this lane's 16 keys, the first `seen`
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      nvk_f32x4(&c4)[4] = sc[t];
+      seen[t] = row_limit[t] - kbase - 16 * g + 1;
+      if (!full) {
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) c4[b][e] = 4 * b + e < seen[t] ? c4[b][e] : -INFINITY;
+      }
+      float mx = nvk_max3(nvk_max3(c4[0][0], c4[0][1], c4[0][2]),
+                          nvk_max3(c4[0][3], c4[1][0], c4[1][1]),
+                          nvk_max3(c4[1][2], c4[1][3], c4[2][0]));
+      mx = nvk_max3(nvk_max3(c4[2][1], c4[2][2], c4[2][3]), mx,
+                    nvk_max3(c4[3][0], c4[3][1], nvk_max3(c4[3][2], c4[3][3], c4[3][3])));
+      mx = nvk_max_xor32(max_xor16(mx));
+      const float m_new = fmaxf(m_run[t], mx * a.scale_log2);
+      const float moff = m_new == -INFINITY ? 0.f : m_new;
+      if (__builtin_amdgcn_ballot_w64(m_new > m_run[t])) {
+        const float alpha = nvk_fast_exp2(m_run[t] - moff);  // 0 while nothing was visible
+        l_part[t][0] *= alpha;
+        l_part[t][1] *= alpha;
+#pragma unroll
+        for (int d = 0; d < HD / 16; ++d) acc[t][d] *= alpha;
+        m_run[t] = m_new;
+      }
 #pragma unroll
       for (int b = 0; b < 4; ++b)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sc[b][e] = 4 * b + e < seen ? sc[b][e] : -INFINITY;
+        for (int e = 0; e < 4; ++e) {
+          c4[b][e] = nvk_fast_exp2(fmaf(c4[b][e], a.scale_log2, -moff));
+          l_part[t][e & 1] += c4[b][e];
+        }
     }
-    float mx = nvk_max3(nvk_max3(sc[0][0], sc[0][1], sc[0][2]),
-                        nvk_max3(sc[0][3], sc[1][0], sc[1][1]),
-                        nvk_max3(sc[1][2], sc[1][3], sc[2][0]));
-    mx = nvk_max3(nvk_max3(sc[2][1], sc[2][2], sc[2][3]), mx,
-                  nvk_max3(sc[3][0], sc[3][1], nvk_max3(sc[3][2], sc[3][3], sc[3][3])));
-    mx = nvk_max_xor32(max_xor16(mx));
-    const float m_new = fmaxf(m_run, mx * a.scale_log2);
-    const float moff = m_new == -INFINITY ? 0.f : m_new;
-    if (__builtin_amdgcn_ballot_w64(m_new > m_run)) {
-      const float alpha = nvk_fast_exp2(m_run - moff);  // 0 while nothing was visible
-      l_part[0] *= alpha;
-      l_part[1] *= alpha;
-#pragma unroll
-      for (int d = 0; d < HD / 16; ++d) acc[d] *= alpha;
-      m_run = m_new;
-    }
-#pragma unroll
-    for (int b = 0; b < 4; ++b)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        sc[b][e] = nvk_fast_exp2(fmaf(sc[b][e], a.scale_log2, -moff));
-        l_part[e & 1] += sc[b][e];
-      }
 
     // ---- O^T += V^T (P vs)^T, one operand per group of dimensions
-    vec8h pf[NS][2];
+    vec8h pf[NT][NS][2];
 #pragma unroll
     for (int i = 0; i < NG; ++i) {
       if (i < NS) {
         const auto* vp = scales(1, g0 + i);
-        nvk_u32x4 vs[2] = {__builtin_bit_cast(nvk_u32x4, vp[0]), __builtin_bit_cast(nvk_u32x4, vp[1])};
-        if (!full) {
-          // a masked key's scale may be anything, what an earlier owner of the page left too
+        const nvk_u32x4 vs[2] = {__builtin_bit_cast(nvk_u32x4, vp[0]),
+                                 __builtin_bit_cast(nvk_u32x4, vp[1])};
 #pragma unroll
-          for (int p = 0; p < 8; ++p) {
-            const int t = seen - 2 * p;
-            vs[p >> 2][p & 3] &= t >= 2 ? 0xffffffffu : t == 1 ? 0xffffu : 0u;
+        for (int t = 0; t < NT; ++t) {
+          nvk_u32x4 vm[2] = {vs[0], vs[1]};
+          if (!full) {
+            // a masked key's scale may be anything, what an earlier owner of the page left too
+#pragma unroll
+            for (int p = 0; p < 8; ++p) {
+              const int n_seen = seen[t] - 2 * p;
+              vm[p >> 2][p & 3] &= n_seen >= 2 ? 0xffffffffu : n_seen == 1 ? 0xffffu : 0u;
+            }
           }
-        }
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          nvk_u32x4 x;
+          for (int h = 0; h < 2; ++h) {
+            nvk_u32x4 x;
 #pragma unroll
-          for (int p = 0; p < 4; ++p)
-            x[p] = times_scales(sc[2 * h + (p >> 1)][2 * (p & 1)], sc[2 * h + (p >> 1)][2 * (p & 1) + 1],
-                                vs[h][p]);
-          pf[i][h] = __builtin_bit_cast(vec8h, x);
+            for (int p = 0; p < 4; ++p)
+              x[p] = times_scales(sc[t][2 * h + (p >> 1)][2 * (p & 1)],
+                                  sc[t][2 * h + (p >> 1)][2 * (p & 1) + 1], vm[h][p]);
+            pf[t][i][h] = __builtin_bit_cast(vec8h, x);
+          }
         }
       }
 #pragma unroll
@@ -517,9 +544,15 @@ __global__ __launch_bounds__(64 * W, W == kWavesPerWG ? 2 : 1) void fp4_attentio
         const i32x2 vc = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
             (__attribute__((address_space(3))) i32x2*)(size_t)(buf + tr_row + 16 * (i ^ sw) +
                                                                 8 * h));
-        acc[d] = NvkElt<true>::mfma16x16x32(fp4_unpack<true>((uint32_t)vc[0]), pf[i % NS][0], acc[d]);
-        acc[d] = NvkElt<true>::mfma16x16x32(fp4_unpack<true>((uint32_t)vc[1]), pf[i % NS][1], acc[d]);
+#pragma unroll
+        for (int k8 = 0; k8 < 2; ++k8) {
+          const vec8h vf = fp4_unpack<true>((uint32_t)vc[k8]);
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+            acc[t][d] = NvkElt<true>::mfma16x16x32(vf, pf[t][i % NS][k8], acc[t][d]);
+        }
       }
+      if constexpr (NT > 1) __builtin_amdgcn_sched_barrier(0);
     }
 
     if (!last) {
@@ -533,31 +566,34 @@ __global__ __launch_bounds__(64 * W, W == kWavesPerWG ? 2 : 1) void fp4_attentio
       continue;
     }
     if (group_end || last) {
-      const float l_tot = nvk_sum_xor32(sum_xor16(l_part[0] + l_part[1]));
-      nvk_f32x4 o[kKeep];
-      kept(o);
-      if (group_end && started_here) {
-        if (row_valid) {
-          const float inv = l_tot == 0.f ? 0.f : 1.f / l_tot;
-          uint16_t* op = a.out + (int64_t)(sq.row0 + tok) * a.out_stride_tok +
-                         (int64_t)head * a.out_stride_head + d0;
 #pragma unroll
-          for (int j = 0; j < kKeep; ++j) {
-            nvk_u32x2 wv;
-            wv.x = E::pack2(o[j][0] * inv, o[j][1] * inv);
-            wv.y = E::pack2(o[j][2] * inv, o[j][3] * inv);
-            *reinterpret_cast<nvk_u32x2*>(op + 16 * j) = wv;
+      for (int t = 0; t < NT; ++t) {
+        const float l_tot = nvk_sum_xor32(sum_xor16(l_part[t][0] + l_part[t][1]));
+        nvk_f32x4 o[kKeep];
+        kept(o, t);
+        if (group_end && started_here) {
+          if (row_valid[t]) {
+            const float inv = l_tot == 0.f ? 0.f : 1.f / l_tot;
+            uint16_t* op = a.out + (int64_t)(sq.row0 + tok[t]) * a.out_stride_tok +
+                           (int64_t)head[t] * a.out_stride_head + d0;
+#pragma unroll
+            for (int j = 0; j < kKeep; ++j) {
+              nvk_u32x2 wv;
+              wv.x = E::pack2(o[j][0] * inv, o[j][1] * inv);
+              wv.y = E::pack2(o[j][2] * inv, o[j][3] * inv);
+              *reinterpret_cast<nvk_u32x2*>(op + 16 * j) = wv;
+            }
           }
-        }
-      } else if (row_valid) {  // the merge reads the valid rows only
-        float* rec =
-            a.rec + ((int64_t)(w * 2 + (started_here ? 0 : 1)) * a.rec_rows + row) * kRec;
+        } else if (row_valid[t]) {  // the merge reads the valid rows only
+          float* rec = a.rec + ((int64_t)(w * 2 + (started_here ? 0 : 1)) * a.rec_rows + kR * t +
+                                row) * kRec;
 #pragma unroll
-        for (int j = 0; j < kKeep; ++j)
-          *reinterpret_cast<nvk_f32x4*>(rec + d0 + 16 * j) = o[j];
-        if (g == 0 && g0 == 0) {
-          rec[HD] = m_run;
-          rec[HD + 1] = l_tot;
+          for (int j = 0; j < kKeep; ++j)
+            *reinterpret_cast<nvk_f32x4*>(rec + d0 + 16 * j) = o[j];
+          if (g == 0 && g0 == 0) {
+            rec[HD] = m_run[t];
+            rec[HD + 1] = l_tot;
+          }
         }
       }
       if (lane == 0) {
@@ -584,19 +620,19 @@ __global__ __launch_bounds__(64 * W, W == kWavesPerWG ? 2 : 1) void fp4_attentio
   if constexpr (WHOLE) {
     // Wave v's rows to LDS (the values' buffers, used up): O, m, l; then a thread sums 4 dimensions of
     // a row over the waves.
-    static_assert(W * (kR / NC) * kRec * 4 <= W * kBuf, "the states fit the buffers");
+    static_assert(NT == 1 && W * (kR / NC) * kRec * 4 <= W * kBuf, "the states fit the buffers");
     float* st = reinterpret_cast<float*>(lds);
-    const float l_tot = nvk_sum_xor32(sum_xor16(l_part[0] + l_part[1]));
+    const float l_tot = nvk_sum_xor32(sum_xor16(l_part[0][0] + l_part[0][1]));
     nvk_f32x4 o[kKeep];
-    kept(o);
+    kept(o, 0);
     wait_reads();
     __syncthreads();
-    if (row_valid) {
+    if (row_valid[0]) {
       float* rec = st + (wave * a.rec_rows + row) * kRec;
 #pragma unroll
       for (int j = 0; j < kKeep; ++j) *reinterpret_cast<nvk_f32x4*>(rec + d0 + 16 * j) = o[j];
       if (g == 0 && g0 == 0) {
-        rec[HD] = m_run;
+        rec[HD] = m_run[0];
         rec[HD + 1] = l_tot;
       }
     }
@@ -648,7 +684,7 @@ __global__ __launch_bounds__(64 * W) void fp4_merge_kernel(AttnArgs a) {
     row0 = sq.row0;
     queries = sq.queries;
   }
-  const int rows = min(queries * a.G - tile * kR, a.rec_rows);  // of this tile
+  const int rows = min(queries * a.G - tile * a.tile_rows, a.rec_rows);  // of this tile
   if (2 * pair >= rows) return;
   const int p1 = desc.x, p2 = desc.y;
   if (p1 >= 0 && p1 == p2) return;  // finished by one wave
@@ -719,7 +755,7 @@ __global__ __launch_bounds__(64 * W) void fp4_merge_kernel(AttnArgs a) {
     }
   }
   if (!ok) return;
-  const int rr = tile * kR + row;
+  const int rr = tile * a.tile_rows + row;
   const int tok = rr / a.G, head = kvh * a.G + rr - tok * a.G;
   const float inv = L == 0.f ? 0.f : 1.f / L;
   nvk_u32x2 wv;
@@ -731,9 +767,24 @@ __global__ __launch_bounds__(64 * W) void fp4_merge_kernel(AttnArgs a) {
 
 // Sizes that follow from a call's static bounds.
 struct Plan {
-  int max_tiles, rec_rows, n_waves, wave_shift;
+  int tile_rows, max_tiles, rec_rows, n_waves, wave_shift;
   size_t desc_bytes, bytes;
 };
+// Tiles of 32 rows: a chunk takes a wave half as long again as with 16, for twice the rows.  That gains
+// where every wave has several chunks, and loses where twice as many tiles share the CUs better.
+// Measured, tiles of 16 / 32 rows, 16/8 heads and (chunks of 32-row tiles per wave, by the table's
+// width):
+//   32 x 9 queries over U{1024..8192} (16) 76.0 / 65.5 us, 32 x 32 (32) 140 / 118, 32 x 64 (64) 265 / 211;
+//   16/16 heads, 16 x 20 over U{2000..4000} (8) 59.5 / 53.1, 16 x 64 (16) 102 / 94;
+//   16/2 heads, 16 x 16 over U{2000..4000} (4) 38.1 / 47.8; 1 x 64 over 8000 (2) 28.4 / 33.4, 1 x 17 (1)
+//   22.9 / 24.4, 1 x 64 over 100 (less) 9.6 / 11.9.
+// An odd number of 16 rows leaves half a tile empty: 16/4 heads, 32 x 12 over U{500..4000} 40.3 / 45.4.
+bool wide_tiles(int64_t rows, int64_t chunks) {
+  const int64_t tiles = (rows + 2 * kR - 1) / (2 * kR);
+  return rows > kR && (rows - 1) / kR % 2 == 1 && tiles <= INT32_MAX / (chunks < 1 ? 1 : chunks) &&
+         tiles * chunks >= 6 * kMaxWGs * kWavesPerWG;
+}
+
 bool plan_of(int batch, int max_queries, int num_q_heads, int num_kv_heads, int head_dim,
              int block_size, int max_blocks, Plan& p) {
   if (batch <= 0 || batch > kMaxBatch || max_queries <= 0 || num_q_heads <= 0 ||
@@ -744,13 +795,14 @@ bool plan_of(int batch, int max_queries, int num_q_heads, int num_kv_heads, int 
   if (G > kR) return false;
   const int64_t rows = (int64_t)max_queries * G;
   const int64_t chunks = ((int64_t)max_blocks * block_size + kCK - 1) / kCK;
-  const int64_t tiles = (rows + kR - 1) / kR;
+  p.tile_rows = wide_tiles(rows, chunks * batch * num_kv_heads) ? 2 * kR : kR;
+  const int64_t tiles = (rows + p.tile_rows - 1) / p.tile_rows;
   if (rows >= 1 << 27 || num_kv_heads > 65535 || chunks > INT32_MAX / kCK ||
       tiles * chunks > INT32_MAX / batch / num_kv_heads ||
       (int64_t)block_size * num_kv_heads * head_dim > INT32_MAX)
     return false;
   p.max_tiles = (int)tiles;
-  p.rec_rows = (int)(rows < kR ? rows : kR);
+  p.rec_rows = (int)(rows < p.tile_rows ? rows : p.tile_rows);
   const int64_t units = tiles * chunks * batch * num_kv_heads;
   p.wave_shift = 2;  // a workgroup's
   while ((1 << p.wave_shift) < units && (1 << p.wave_shift) < kMaxWGs * kWavesPerWG) ++p.wave_shift;
@@ -785,24 +837,26 @@ int launch(const AttnArgs& a, hipStream_t s) {
   const std::false_type no;
   if (whole_groups(a.n_query * a.G, HD, (int64_t)a.batch * a.num_kv_heads, a.cap)) {
     const auto one_kernel = [&](auto one) {
-      hipLaunchKernelGGL((fp4_attention_kernel<HD, F16, decltype(one)::value, NG, kWholeWaves, true>),
+      hipLaunchKernelGGL((fp4_attention_kernel<HD, F16, decltype(one)::value, NG, 1, kWholeWaves, true>),
                          dim3(a.num_kv_heads, a.batch), dim3(64 * kWholeWaves), 0, s, a);
     };
     a.block_size % kCK ? one_kernel(no) : one_kernel(yes);
     return nvk_launch_status();
   }
-  const auto main = [&](auto nc) {
+  const auto main = [&](auto nc, auto nt) {
+    constexpr int NC = decltype(nc)::value, NT = decltype(nt)::value;
     if (a.block_size % kCK)
-      hipLaunchKernelGGL((fp4_attention_kernel<HD, F16, false, decltype(nc)::value>), grid, block, 0,
-                         s, a);
+      hipLaunchKernelGGL((fp4_attention_kernel<HD, F16, false, NC, NT>), grid, block, 0, s, a);
     else
-      hipLaunchKernelGGL((fp4_attention_kernel<HD, F16, true, decltype(nc)::value>), grid, block, 0, s,
-                         a);
+      hipLaunchKernelGGL((fp4_attention_kernel<HD, F16, true, NC, NT>), grid, block, 0, s, a);
   };
+  const std::integral_constant<int, 1> c1;
+  const std::integral_constant<int, 2> c2;
   const int rows = a.n_query * a.G;
-  if (rows <= kR / NG) main(std::integral_constant<int, NG>{});
-  else if (rows <= kR / 2) main(std::integral_constant<int, 2>{});
-  else main(std::integral_constant<int, 1>{});
+  if (rows <= kR / NG) main(std::integral_constant<int, NG>{}, c1);
+  else if (rows <= kR / 2) main(c2, c1);
+  else if (a.tile_rows == kR) main(c1, c1);
+  else main(c1, c2);
   const int st = nvk_launch_status();
   if (st != NVK_OK) return st;
   const dim3 mgrid(a.max_tiles * ((a.rec_rows + 1) / 2), a.num_kv_heads, a.batch);
@@ -1001,6 +1055,7 @@ extern "C" int nvk_fp4_attention(const void* q, int64_t q_stride_tok, int64_t q_
   a.bt_stride = bt_stride;
   a.batch = batch;
   a.n_query = max_seqlen_q;
+  a.tile_rows = p.tile_rows;
   a.max_tiles = p.max_tiles;
   a.cap = max_blocks * block_size;
   a.block_size = block_size;

@@ -104,6 +104,42 @@ def test_ragged_queries(news, cached, bs, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("n,hq,hkv,d,bs", [(9, 16, 8, 128, 64), (16, 16, 8, 128, 16),
+                                           (60, 16, 8, 128, 256), (30, 8, 8, 64, 64),
+                                           (4, 64, 8, 64, 16), (25, 8, 8, 128, 48)])
+def test_tiles_of_32_rows(n, hq, hkv, d, bs, dtype):
+    """Tables that could hold 32768 tokens of each sequence: many chunks for every wave, by which tiles
+    of 32 rows are chosen, over contexts that end anywhere."""
+    lens = [n, n + 1, 64, 300, 130, n - 1, 0, 1000]
+    tables, nb = tables_of(lens, bs, 4)
+    wide = np.full((len(lens), 32768 // bs), -1, np.int32)
+    wide[:, :tables.shape[1]] = tables
+    pages = Pages(7, nb, bs, hkv, d, dtype)
+    q = rng_rows(11, (len(lens), n, hq, d), dtype).cuda()
+    say(f"fp4 tiles of 32 rows: {n} queries {hq}/{hkv} x {d} pages {bs} {dtype}")
+    out = flash_attn_with_kvcache(q, *pages.gpu(), cache_seqlens=_int(lens), block_table=_int(wide),
+                                  causal=True)
+    ref, size = _reference(q.flatten(0, 1), pages, tables, [n] * len(lens), lens, d ** -0.5)
+    assert_close(out, ref, size, dtype, "fp4 tiles of 32 rows")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("hq,hkv,d,bs", [(16, 8, 128, 256), (4, 1, 128, 16), (16, 16, 64, 48)])
+def test_one_workgroup_per_group_and_ranges_of_waves_agree(hq, hkv, d, bs, dtype):
+    """Short contexts in one kernel; the same with a table that could hold more, cut between waves."""
+    lens = [1, 0, 64, 700, 1000, 65]
+    tables, nb = tables_of(lens, bs, 4)
+    pages = Pages(7, nb, bs, hkv, d, dtype)
+    q = rng_rows(11, (len(lens), hq, d), dtype).cuda()
+    ref, size = _reference(q, pages, tables, [1] * len(lens), lens, d ** -0.5)
+    for width in (tables.shape[1], 8192 // bs):
+        wide = np.full((len(lens), width), -1, np.int32)
+        wide[:, :tables.shape[1]] = tables
+        out = paged_decode(q, *pages.gpu(), _int(lens), _int(wide), None)
+        assert_close(out, ref, size, dtype, f"fp4 decode, tables of {width} pages")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
 @pytest.mark.parametrize("hq,hkv,bs", [(2, 2, 256), (4, 2, 16), (4, 1, 64), (8, 1, 48), (3, 1, 64)])
 def test_chunks_of_many_queries(hq, hkv, bs, dtype):
     """Over f16 pages (three heads per kv head: without), with chunks that end inside a tile, in front
