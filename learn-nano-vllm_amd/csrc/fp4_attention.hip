@@ -7,10 +7,10 @@
 // The codes kc, vc are exact in bf16 and f16, so they are what the matrix instructions multiply, and
 // the scales are applied to the products: to the f32 sums of a key's groups (S), and to
 // the probabilities (P.V), which become one operand per group.
-//   * A wave owns 16 rows (query token x query head of a kv head) and streams their keys in chunks
-//     of 64; the chunks of all (sequence, kv head, 16-row tile) groups are cut into equal
+//   * A wave owns a tile of 16 or 32 rows (query token x query head of a kv head) and streams their
+//     keys in chunks of 64; the chunks of all (sequence, kv head, tile) groups are cut into equal
 //     contiguous ranges, one per wave.  Groups cut between waves leave (O, m, l) records that a
-//     second kernel merges.
+//     second kernel merges.  A few short groups of a few rows get a workgroup of 16 waves each instead.
 //   * S^T = K Q^T on v_mfma_f32_16x16x32: operand row m = 4 a + i of key block b is key
 //     16 a + 4 b + i of the chunk, so lane (g, r) ends up with the scores of keys 16 g .. +15 of
 //     row r in order: the order in which ds_read_b64_tr_b4 hands it the values of a dimension.
@@ -22,6 +22,10 @@
 //     loaded once the scores have used these, its values and scales after P.V: there is always
 //     something in flight, and a second buffer for what goes to LDS gained nothing (64 x
 //     U{100..2048}, 16/8 heads: 23.1 us per call with two, 22.3 with one).
+// What bounds it.  64 x U{100..2048} keys, 16/8 heads (86 MB of codes and scales), 22 us: 4 us until the
+// first chunk has come (prefix, position, page, data: four dependent round trips), 11 to 12 us of
+// stream at 5.7 to 6.4 TB/s, 3.7 us for the merging kernel and its launch.  Loads alone take 15.5 us;
+// without the 128 conversions of a chunk the whole is 1 % shorter, so it is not the arithmetic.
 #include <type_traits>
 
 #include "fp4.h"
@@ -785,22 +789,27 @@ bool wide_tiles(int64_t rows, int64_t chunks) {
          tiles * chunks >= 6 * kMaxWGs * kWavesPerWG;
 }
 
-bool plan_of(int batch, int max_queries, int num_q_heads, int num_kv_heads, int head_dim,
-             int block_size, int max_blocks, Plan& p) {
+// What either route takes.
+bool sizes_ok(int batch, int max_queries, int num_q_heads, int num_kv_heads, int head_dim,
+              int block_size, int max_blocks) {
   if (batch <= 0 || batch > kMaxBatch || max_queries <= 0 || num_q_heads <= 0 ||
       num_kv_heads <= 0 || num_q_heads % num_kv_heads || block_size <= 0 || max_blocks <= 0)
     return false;
   if ((head_dim != 128 && head_dim != 64) || block_size % 16) return false;
   const int G = num_q_heads / num_kv_heads;
-  if (G > kR) return false;
-  const int64_t rows = (int64_t)max_queries * G;
+  return G <= kR && num_kv_heads <= 65535 && (int64_t)max_queries * G < 1 << 27 &&
+         (int64_t)max_blocks * block_size <= INT32_MAX - kCK &&
+         (int64_t)block_size * num_kv_heads * head_dim <= INT32_MAX;
+}
+
+// Of sizes that are ok.  False: more (tile, chunk) pairs than the split counts in 32 bits.
+bool plan_of(int batch, int max_queries, int num_q_heads, int num_kv_heads, int head_dim,
+             int block_size, int max_blocks, Plan& p) {
+  const int64_t rows = (int64_t)max_queries * (num_q_heads / num_kv_heads);
   const int64_t chunks = ((int64_t)max_blocks * block_size + kCK - 1) / kCK;
   p.tile_rows = wide_tiles(rows, chunks * batch * num_kv_heads) ? 2 * kR : kR;
   const int64_t tiles = (rows + p.tile_rows - 1) / p.tile_rows;
-  if (rows >= 1 << 27 || num_kv_heads > 65535 || chunks > INT32_MAX / kCK ||
-      tiles * chunks > INT32_MAX / batch / num_kv_heads ||
-      (int64_t)block_size * num_kv_heads * head_dim > INT32_MAX)
-    return false;
+  if (tiles * chunks > INT32_MAX / batch / num_kv_heads) return false;
   p.max_tiles = (int)tiles;
   p.rec_rows = (int)(rows < p.tile_rows ? rows : p.tile_rows);
   const int64_t units = tiles * chunks * batch * num_kv_heads;
@@ -820,7 +829,7 @@ bool plan_of(int batch, int max_queries, int num_q_heads, int num_kv_heads, int 
 //   1 x 100 keys 7.8 / 6.0 us, 1 x 1000 8.7 / 7.7, 4 x 1024 9.4 / 8.5, 32 x U{100..1000} 14.3 / 10.1;
 //   1 x 1280 8.7 / 10.6, 1 x 2048 9.2 / 12.0, 4 x 2048 10.1 / 12.5 (called one by one: 16.3 / 13.6), 8 x
 //   2048 12.5 / 12.8, 12 x 2048 14.8 / 13.2, 32 x 2048 21.3 / 17.8;
-//   16 x U{100..3072} 16.1 / 17.4, 32 x U{100..3072} 18.9 / 19.1;
+//   32 x U{100..4096} 23.7 / 23.6, 32 x 4096 33.5 / 30.0;
 //   33 x U{100..256} (264 groups) 9.2 / 10.3, 64 x U{100..300} 11.9 / 14.6.
 constexpr int kWholeWaves = 16;
 constexpr int64_t kWholeGroups = 256, kWholeKeys = 1024, kWholeMinGroups = 32;
@@ -874,10 +883,11 @@ int launch(const AttnArgs& a, hipStream_t s) {
 }
 
 // Long query ranges go through f16 pages (fp4.h).
-#ifndef NVK_FP4_DIRECT_ROWS
-#define NVK_FP4_DIRECT_ROWS 128
-#endif
-constexpr int kDirectRows = NVK_FP4_DIRECT_ROWS;  // rows per kv head that the kernel above takes itself
+// From 129 rows (queries x G) per kv head on.  Measured, the kernel above / pages, 16/8 heads:
+//   128 rows: 32 x 64 queries over U{1024..8192} 210 / 348 us, 1 x 64 over 8000 29 / 37, 4 x 64 over 300
+//   18.5 / 18.6; 192: 398 / 428 (tiles of 16 rows), 35.6 / 36.5, 22.3 / 18.6; 256: 524 / 434, 41.5 / 36.9,
+//   16/4 heads, 8 x 64 over 2000 43.5 / 36.2, 16/16 heads, 16 x 192 (192 rows) 279 / 254.
+constexpr int kDirectRows = 128;
 constexpr int64_t kPageBytesMost = (int64_t)512 << 20;  // pages of a part of the batch (one sequence: any)
 
 // Workspace of that route, for `part` sequences at a time.
@@ -995,12 +1005,14 @@ extern "C" size_t nvk_fp4_attention_workspace_size(int32_t batch, int32_t max_se
                                                    int32_t block_size, int32_t max_blocks) {
   Plan p;
   PagePlan pp;
-  if (!plan_of(batch, max_seqlen_q, num_q_heads, num_kv_heads, head_dim, block_size, max_blocks, p))
+  if (!sizes_ok(batch, max_seqlen_q, num_q_heads, num_kv_heads, head_dim, block_size, max_blocks))
     return 0;
-  return page_plan(batch, max_seqlen_q, max_seqlen_k, num_q_heads, num_kv_heads, head_dim,
-                   block_size, max_blocks, pp)
-             ? pp.bytes
-             : p.bytes;
+  if (page_plan(batch, max_seqlen_q, max_seqlen_k, num_q_heads, num_kv_heads, head_dim, block_size,
+                max_blocks, pp))
+    return pp.bytes;
+  return plan_of(batch, max_seqlen_q, num_q_heads, num_kv_heads, head_dim, block_size, max_blocks, p)
+             ? p.bytes
+             : 0;
 }
 
 extern "C" int nvk_fp4_attention(const void* q, int64_t q_stride_tok, int64_t q_stride_head,
@@ -1022,9 +1034,15 @@ extern "C" int nvk_fp4_attention(const void* q, int64_t q_stride_tok, int64_t q_
   if (batch == 0 || total_q == 0 || max_seqlen_q == 0) return NVK_OK;
   if (total_q > INT32_MAX) return NVK_EINVAL;
   if (!cu_seqlens_q && (int64_t)batch * max_seqlen_q != total_q) return NVK_EINVAL;
-  Plan p;
-  if (num_blocks == 0 || !plan_of(batch, max_seqlen_q, num_q_heads, num_kv_heads, head_dim,
-                                  block_size, max_blocks, p))
+  Plan p{};
+  PagePlan pp;
+  if (num_blocks == 0 || !sizes_ok(batch, max_seqlen_q, num_q_heads, num_kv_heads, head_dim,
+                                   block_size, max_blocks))
+    return NVK_EUNSUPPORTED;
+  const bool pages = page_plan(batch, max_seqlen_q, max_seqlen_k, num_q_heads, num_kv_heads,
+                               head_dim, block_size, max_blocks, pp);
+  if (!pages && !plan_of(batch, max_seqlen_q, num_q_heads, num_kv_heads, head_dim, block_size,
+                         max_blocks, p))
     return NVK_EUNSUPPORTED;
   if (!q || !k_data || !k_scale || !v_data || !v_scale || !seqlens_k || !block_tables || !out)
     return NVK_EINVAL;
@@ -1035,9 +1053,6 @@ extern "C" int nvk_fp4_attention(const void* q, int64_t q_stride_tok, int64_t q_
   if ((uintptr_t)out % 8 || out_stride_tok % 4 || out_stride_head % 4) return NVK_EALIGN;
   if (((uintptr_t)cu_seqlens_q | (uintptr_t)seqlens_k | (uintptr_t)block_tables) % 4)
     return NVK_EALIGN;
-  PagePlan pp;
-  const bool pages = page_plan(batch, max_seqlen_q, max_seqlen_k, num_q_heads, num_kv_heads,
-                               head_dim, block_size, max_blocks, pp);
   if (!workspace || workspace_bytes < (pages ? pp.bytes : p.bytes)) return NVK_EWORKSPACE;
   if ((uintptr_t)workspace % 256) return NVK_EALIGN;
   AttnArgs a{};
