@@ -554,9 +554,11 @@ int nvk_sample(const void* logits, int64_t row_stride, int32_t batch, int32_t vo
  * nvk_fp4_store: nvk_kv_store into such caches: row slot_mapping[t] of every head = what the
  *   format makes of key[t], value[t] (row t at t * row_stride, heads contiguous; rows 16-byte
  *   aligned, strides multiples of 8 elements).  Slots outside [0, num_blocks * block_size)
- *   are skipped; of several tokens with one slot one wins.
+ *   are skipped.  Several tokens with one slot are a race, never a fault: that
+ *   row's codes and scales may come from different ones.
  * nvk_fp4_load: key[t], value[t] = the rows of slot_mapping[t], every value rounded once to dtype;
- *   zeros where the slot lies outside the cache.
+ *   zeros where the slot lies outside the cache.  code * scale can be past f16's largest by a
+ *   step of the scale (6 * 10920 = 65520): an infinity in f16.
  * Each is one kernel.
  */
 int nvk_fp4_store(const void* key, int64_t key_row_stride, const void* value,

@@ -9,8 +9,8 @@
 // e2m1: sign, then 0, 0.5, 1, 1.5, 2, 3, 4, 6: what gfx950 converts to bf16 and f16, two
 // codes per instruction and exactly.  The scale of 32 dimensions is f16(min(max|x| / 6, 65504)):
 // 16 bits of it cost 0.5 bit per value, and keep the grid's top at the largest value, where a power
-// of two (one byte) would leave up to half of the grid unused (rms error of N(0, 1) values: 0.094
-// with this scale, 0.125 with powers of two).  f16 rather than bf16: v_fma_mix takes it as it is.
+// of two (one byte) would leave up to half of the grid unused (rms error of N(0, 1) values: 0.101
+// with this scale, 0.115 with the best rule for powers of two).  f16 rather than bf16: v_fma_mix takes it as it is.
 //
 // A row of values holds its dimensions in order.  A row of keys holds them in units of 8
 // (4 bytes): unit 32 s + 8 g .. + 7 at place (D / 32) g + s, so that the 16 (D = 64: 8) bytes that
