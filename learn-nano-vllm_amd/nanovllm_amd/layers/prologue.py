@@ -26,8 +26,8 @@ from __future__ import annotations
 import torch
 
 from nanovllm_amd import _lib
-from nanovllm_amd.fp4_cache import Fp4Cache
-from nanovllm_amd.flash_api import _int32, _key_bound
+from nanovllm_amd.fp4_cache import Fp4Cache, fp4_store
+from nanovllm_amd.flash_api import _int32, _key_bound, paged_decode
 from nanovllm_amd.layers.attention import Attention, _prefill_order
 from nanovllm_amd.utils.context import get_context
 
@@ -105,8 +105,14 @@ def qk_norm_rope_store(positions: torch.Tensor, qkv: torch.Tensor, num_heads: in
     k [T, Hkv, D] new tensor or None when return_k is False, v = the view of
     qkv the reference passes on).  With slot_mapping given, the rotated k and
     the raw v rows are stored into the caches (slot -1 skipped), as
-    store_kvcache does; without it nothing is stored.
+    store_kvcache does; without it nothing is stored.  Into ``Fp4Cache`` caches
+    they are stored by a second kernel.
     """
+    if slot_mapping is not None and (isinstance(k_cache, Fp4Cache) or isinstance(v_cache, Fp4Cache)):
+        q, k, v = qk_norm_rope_store(positions, qkv, num_heads, num_kv_heads, head_dim,
+                                     q_norm_weight, k_norm_weight, eps, cos_sin_cache)
+        fp4_store(k, v, k_cache, v_cache, slot_mapping)
+        return q, k if return_k else None, v
     T = qkv.shape[0]
     cs, pos, slots, cache_slots = _check_prologue(
         positions, qkv, num_heads, num_kv_heads, head_dim, q_norm_weight, k_norm_weight,
@@ -145,7 +151,12 @@ def paged_decode_with_prologue(positions: torch.Tensor, qkv: torch.Tensor, num_h
     scale)``.  Row b of qkv is sequence b's new
     token; ``slot_mapping[b]`` must be the cache row of key
     ``context_lens[b] - 1`` (as model_runner.prepare_decode builds them).
-    Returns [B, Hq, D] (or fills ``out``)."""
+    Returns [B, Hq, D] (or fills ``out``).  ``Fp4Cache`` caches take the two calls."""
+    if isinstance(k_cache, Fp4Cache) or isinstance(v_cache, Fp4Cache):
+        q, _, _ = qk_norm_rope_store(positions, qkv, num_heads, num_kv_heads, head_dim,
+                                     q_norm_weight, k_norm_weight, eps, cos_sin_cache, k_cache,
+                                     v_cache, slot_mapping, return_k=False)
+        return paged_decode(q, k_cache, v_cache, context_lens, block_tables, scale, out=out)
     B = qkv.shape[0]
     q_size, kv_size = num_heads * head_dim, num_kv_heads * head_dim
     assert qkv.dim() == 2 and qkv.shape[1] == q_size + 2 * kv_size and qkv.stride(-1) == 1

@@ -8,7 +8,8 @@ import torch
 from fp4_utils import assert_close
 from gpu_utils import say
 from nanovllm_amd import (Attention, Fp4Cache, attention_with_prologue, flash_attn_with_kvcache,
-                          qk_norm_rope_store, rope_cos_sin_cache, store_kvcache)
+                          paged_decode_with_prologue, qk_norm_rope_store, rope_cos_sin_cache,
+                          store_kvcache)
 from nanovllm_amd.engine.graph_runner import DecodeGraphRunner
 from nanovllm_amd.utils.context import reset_context, set_context
 from oracle import fp4_oracle as orc
@@ -195,3 +196,32 @@ def test_decode_steps_replayed_as_a_graph():
             assert_close(out.view(live, HQ, HD), ref, size, "bf16", f"fp4 graph, {live} live")
     finally:
         reset_context()
+
+
+def test_the_prologue_s_own_calls_take_the_caches():
+    """qk_norm_rope_store and paged_decode_with_prologue into 4-bit caches are the calls that they
+    stand for."""
+    m = _Model()
+    lens = [5, 300, 512]
+    qkv = m.qkv(3)
+    pos = torch.tensor([n - 1 for n in lens], device="cuda")
+    slots = torch.tensor([TABLES[b][(n - 1) // BS] * BS + (n - 1) % BS for b, n in enumerate(lens)],
+                         dtype=torch.int32, device="cuda")
+    args = (pos, qkv, HQ, HKV, HD, m.q_norm.weight, m.k_norm.weight, 1e-6, m.rope.cos_sin_cache)
+    caches = [[Fp4Cache.zeros(NB, BS, HKV, HD) for _ in range(2)] for _ in range(3)]
+    q, k, v = qk_norm_rope_store(*args)
+    store_kvcache(k, v, *caches[0], slots)
+    got = qk_norm_rope_store(*args, *caches[1], slots)
+    assert all(torch.equal(a, b) for a, b in zip(got, (q, k, v)))
+    assert qk_norm_rope_store(*args, *caches[1], slots, return_k=False)[1] is None
+    lens = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    tables = torch.tensor(TABLES, dtype=torch.int32, device="cuda")
+    want = flash_attn_with_kvcache(q.unsqueeze(1), *caches[0], cache_seqlens=lens,
+                                   block_table=tables, softmax_scale=SCALE, causal=True)
+    out = torch.empty(3, HQ, HD, dtype=torch.bfloat16, device="cuda")
+    paged_decode_with_prologue(*args, *caches[2], slots, lens, tables, SCALE, out=out)
+    assert torch.equal(out, want[:, 0])
+    for pair in caches[1:]:
+        for c, ref in zip(pair, caches[0]):
+            assert torch.equal(c.data, ref.data) and torch.equal(c.scale, ref.scale)
+    say("prologue calls over 4-bit caches ok")
