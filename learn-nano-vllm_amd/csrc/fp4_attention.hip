@@ -59,8 +59,8 @@ struct AttnArgs {
   float scale_log2;
   uint16_t* out;
   int64_t out_stride_tok, out_stride_head;
-  int32_t* desc;  // [batch][Hkv][max_tiles] x 2: first and last wave of the group, -1 if empty
-  float* rec;     // [n_waves][2][rec_rows][HD + 4]: O, m, l
+  int32_t* desc;  // [batch][Hkv][max_tiles] x 2: first and last workgroup of the group, -1 if empty
+  float* rec;     // [workgroups][2][rec_rows][HD + 4]: O, m, l
   int rec_rows, n_waves, wave_shift;  // n_waves = 2^wave_shift
 };
 
@@ -213,6 +213,11 @@ __global__ __launch_bounds__(64 * W, W == kWavesPerWG ? 2 : 1) void fp4_attentio
   __shared__ __attribute__((aligned(1024))) uint8_t lds[W * kBuf];
   __shared__ int s_cs[WHOLE ? 1 : kMaxBatch + 1];
   __shared__ int s_wsum[kWavesPerWG];
+  // !WHOLE: what waves 1 .. W - 1 hold of a group that began before them: O, (m, l), whether it ended there
+  constexpr int kFollow = WHOLE ? 1 : W - 1;
+  __shared__ nvk_f32x4 s_o[kFollow][WHOLE ? 1 : NT * 2 * NS][64];
+  __shared__ float2 s_ml[kFollow][NT][64];
+  __shared__ int s_ended[kFollow];
   const int tid = threadIdx.x, lane = tid & 63;
   const int r = lane & 15, g = lane >> 4;
   const int Hkv = a.num_kv_heads;
@@ -248,10 +253,12 @@ __global__ __launch_bounds__(64 * W, W == kWavesPerWG ? 2 : 1) void fp4_attentio
   }
   const Split sp{T, T < a.n_waves ? T : a.n_waves, a.wave_shift};
   if constexpr (!WHOLE) {
-    if (w >= sp.P) return;
+    if (w >= sp.P) {  // no chunk
+      __syncthreads();  // the join's
+      return;
+    }
     c0 = sp.begin(w);
     c1 = sp.begin(w + 1);
-    if (c0 >= c1) return;
     s = nvk_last_le(s_cs, a.batch, Hkv, c0, lane);
     sq = seq_of(a, s);
     n = uniform(chunks_of(sq));
@@ -387,8 +394,35 @@ __global__ __launch_bounds__(64 * W, W == kWavesPerWG ? 2 : 1) void fp4_attentio
     }
   };
 
+  auto put_rows = [&](const nvk_f32x4 (&o)[kKeep], float l, int t) {
+    if (!row_valid[t]) return;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    uint16_t* op = a.out + (int64_t)(sq.row0 + tok[t]) * a.out_stride_tok +
+                   (int64_t)head[t] * a.out_stride_head + d0;
+#pragma unroll
+    for (int j = 0; j < kKeep; ++j) {
+      nvk_u32x2 wv;
+      wv.x = E::pack2(o[j][0] * inv, o[j][1] * inv);
+      wv.y = E::pack2(o[j][2] * inv, o[j][3] * inv);
+      *reinterpret_cast<nvk_u32x2*>(op + 16 * j) = wv;
+    }
+  };
+  // The workgroup's record of the group that goes on behind it (0), or began before it (1).
+  auto put_record = [&](const nvk_f32x4 (&o)[kKeep], float m, float l, int t) {
+    if (!row_valid[t]) return;  // the merge reads the valid rows only
+    float* rec = a.rec + ((int64_t)(blockIdx.x * 2 + (started_here ? 0 : 1)) * a.rec_rows + kR * t +
+                          row) * kRec;
+#pragma unroll
+    for (int j = 0; j < kKeep; ++j) *reinterpret_cast<nvk_f32x4*>(rec + d0 + 16 * j) = o[j];
+    if (g == 0 && g0 == 0) {
+      rec[HD] = m;
+      rec[HD + 1] = l;
+    }
+  };
+
   kvec kraw[4];
   Where at;
+  bool cut = false;  // the range ends inside a group
   if (!WHOLE || c0 < c1) {
     at = locate(sq.keys, s, kvh, k);
     issue_keys(at, kraw);
@@ -565,6 +599,7 @@ __global__ __launch_bounds__(64 * W, W == kWavesPerWG ? 2 : 1) void fp4_attentio
     }
 
     // ---- the group's or the range's end
+    cut = last && !group_end;
     if (WHOLE) {
       ++k;
       continue;
@@ -576,37 +611,23 @@ __global__ __launch_bounds__(64 * W, W == kWavesPerWG ? 2 : 1) void fp4_attentio
         nvk_f32x4 o[kKeep];
         kept(o, t);
         if (group_end && started_here) {
-          if (row_valid[t]) {
-            const float inv = l_tot == 0.f ? 0.f : 1.f / l_tot;
-            uint16_t* op = a.out + (int64_t)(sq.row0 + tok[t]) * a.out_stride_tok +
-                           (int64_t)head[t] * a.out_stride_head + d0;
+          put_rows(o, l_tot, t);
+        } else if (!started_here && wave > 0) {
 #pragma unroll
-            for (int j = 0; j < kKeep; ++j) {
-              nvk_u32x2 wv;
-              wv.x = E::pack2(o[j][0] * inv, o[j][1] * inv);
-              wv.y = E::pack2(o[j][2] * inv, o[j][3] * inv);
-              *reinterpret_cast<nvk_u32x2*>(op + 16 * j) = wv;
-            }
-          }
-        } else if (row_valid[t]) {  // the merge reads the valid rows only
-          float* rec = a.rec + ((int64_t)(w * 2 + (started_here ? 0 : 1)) * a.rec_rows + kR * t +
-                                row) * kRec;
-#pragma unroll
-          for (int j = 0; j < kKeep; ++j)
-            *reinterpret_cast<nvk_f32x4*>(rec + d0 + 16 * j) = o[j];
-          if (g == 0 && g0 == 0) {
-            rec[HD] = m_run[t];
-            rec[HD + 1] = l_tot;
-          }
+          for (int j = 0; j < kKeep; ++j) s_o[wave - 1][t * kKeep + j][lane] = o[j];
+          s_ml[wave - 1][t][lane] = make_float2(m_run[t], l_tot);
+          if (lane == 0) s_ended[wave - 1] = group_end;
+        } else if (group_end) {
+          put_record(o, m_run[t], l_tot, t);
         }
       }
       if (lane == 0) {
         const int first = Hkv * s_cs[s] + (kvh * tiles + tile) * n;
         const int64_t e = ((int64_t)s * Hkv + kvh) * a.max_tiles + tile;
         *reinterpret_cast<int2*>(a.desc + 2 * e) =
-            make_int2(sp.owner(first), sp.owner(first + n - 1));
+            make_int2(sp.owner(first) / W, sp.owner(first + n - 1) / W);
       }
-      if (last) return;
+      if (last) break;
       s = ns;
       sq = nsq;
       kvh = nkvh;
@@ -621,7 +642,38 @@ __global__ __launch_bounds__(64 * W, W == kWavesPerWG ? 2 : 1) void fp4_attentio
     }
   }
 
-  if constexpr (WHOLE) {
+  if constexpr (!WHOLE) {
+    // A group that is cut between waves of the workgroup: the first of them joins what the others hold.
+    __syncthreads();
+    if (!cut || (!started_here && wave > 0)) return;
+    bool ended = false;
+    nvk_f32x4 o[NT][kKeep];
+    float l[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      l[t] = nvk_sum_xor32(sum_xor16(l_part[t][0] + l_part[t][1]));
+      kept(o[t], t);
+    }
+    for (int v = wave + 1; v < W && !ended; ++v) {
+      ended = uniform(s_ended[v - 1]);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const float2 ml = s_ml[v - 1][t][lane];
+        const float m = fmaxf(m_run[t], ml.x), mref = m == -INFINITY ? 0.f : m;
+        const float w0 = nvk_fast_exp2(m_run[t] - mref), w1 = nvk_fast_exp2(ml.x - mref);
+        m_run[t] = m;
+        l[t] = l[t] * w0 + ml.y * w1;
+#pragma unroll
+        for (int j = 0; j < kKeep; ++j) o[t][j] = o[t][j] * w0 + s_o[v - 1][t * kKeep + j][lane] * w1;
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+      if (started_here && ended)
+        put_rows(o[t], l[t], t);
+      else
+        put_record(o[t], m_run[t], l[t], t);
+  } else {
     // Wave v's rows to LDS (the values' buffers, used up): O, m, l; then a thread sums 4 dimensions of
     // a row over the waves.
     static_assert(NT == 1 && W * (kR / NC) * kRec * 4 <= W * kBuf, "the states fit the buffers");
@@ -691,7 +743,7 @@ __global__ __launch_bounds__(64 * W) void fp4_merge_kernel(AttnArgs a) {
   const int rows = min(queries * a.G - tile * a.tile_rows, a.rec_rows);  // of this tile
   if (2 * pair >= rows) return;
   const int p1 = desc.x, p2 = desc.y;
-  if (p1 >= 0 && p1 == p2) return;  // finished by one wave
+  if (p1 >= 0 && p1 == p2) return;  // finished by one workgroup
   const int half = lane / kLanes, d0 = 4 * (lane % kLanes);
   const bool ok = half < 2 && 2 * pair + half < rows;
   const int row = ok ? 2 * pair + half : 2 * pair;
@@ -817,7 +869,8 @@ bool plan_of(int batch, int max_queries, int num_q_heads, int num_kv_heads, int 
   while ((1 << p.wave_shift) < units && (1 << p.wave_shift) < kMaxWGs * kWavesPerWG) ++p.wave_shift;
   p.n_waves = 1 << p.wave_shift;
   p.desc_bytes = ((size_t)batch * num_kv_heads * tiles * 8 + 255) / 256 * 256;
-  p.bytes = p.desc_bytes + (size_t)p.n_waves * 2 * p.rec_rows * (head_dim + 4) * sizeof(float);
+  p.bytes = p.desc_bytes + (size_t)p.n_waves / kWavesPerWG * 2 * p.rec_rows * (head_dim + 4) *
+                               sizeof(float);
   return true;
 }
 
@@ -872,7 +925,8 @@ int launch(const AttnArgs& a, hipStream_t s) {
   // By the parts that a group has on average, where it has any: a wave fetches 4 in a round trip.
   // 64 x U{100..2048} keys, 16/8 heads (4 parts): 24.4 us with one wave per row pair, 23.1 with four; 32
   // x 6 over U{1024..8192} (8 parts): 42.7 with one, 42.1 with four or sixteen.
-  const int64_t parts = a.n_waves / ((int64_t)a.batch * a.num_kv_heads * a.max_tiles);
+  const int64_t parts =
+      a.n_waves / kWavesPerWG / ((int64_t)a.batch * a.num_kv_heads * a.max_tiles);
   if (parts >= 16)
     hipLaunchKernelGGL((fp4_merge_kernel<HD, F16, 16>), mgrid, dim3(64 * 16), 0, s, a);
   else if (parts >= 4)
