@@ -9,8 +9,10 @@
 // the probabilities (P.V), which become one operand per group.
 //   * A wave owns a tile of 16 or 32 rows (query token x query head of a kv head) and streams their
 //     keys in chunks of 64; the chunks of all (sequence, kv head, tile) groups are cut into equal
-//     contiguous ranges, one per wave.  Groups cut between waves leave (O, m, l) records that a
-//     second kernel merges.  A few short groups of a few rows get a workgroup of 16 waves each instead.
+//     contiguous ranges, one per wave.  The waves of a workgroup join a group that is cut between
+//     them in LDS; one cut between workgroups leaves (O, m, l) records that a second kernel merges.
+//     (Records of every wave: 192 x U{256..4096} keys, 16/2 heads, 34.1 us and not 31.6, 8 x 16 queries
+//     over 2000 27.1 and not 19.1.)  A few short groups of a few rows get a workgroup of 16 waves each.
 //   * S^T = K Q^T on v_mfma_f32_16x16x32: operand row m = 4 a + i of key block b is key
 //     16 a + 4 b + i of the chunk, so lane (g, r) ends up with the scores of keys 16 g .. +15 of
 //     row r in order: the order in which ds_read_b64_tr_b4 hands it the values of a dimension.
@@ -24,8 +26,9 @@
 //     U{100..2048}, 16/8 heads: 23.1 us per call with two, 22.3 with one).
 // What bounds it.  64 x U{100..2048} keys, 16/8 heads (86 MB of codes and scales), 22 us: 4 us until the
 // first chunk has come (prefix, position, page, data: four dependent round trips), 11 to 12 us of
-// stream at 5.7 to 6.4 TB/s, 3.7 us for the merging kernel and its launch.  Loads alone take 15.5 us;
-// without the 128 conversions of a chunk the whole is 1 % shorter, so it is not the arithmetic.
+// stream at 5.7 to 6.4 TB/s, 4 us for the merging kernel and its launch.  Without the 128 conversions
+// of a chunk it is 1 % shorter, so it is not the arithmetic.  192 x U{256..4096}, 16/16 heads (922
+// MB): 154 us, 6.0 TB/s.
 #include <type_traits>
 
 #include "fp4.h"
@@ -830,11 +833,12 @@ struct Plan {
 // where every wave has several chunks, and loses where twice as many tiles share the CUs better.
 // Measured, tiles of 16 / 32 rows, 16/8 heads and (chunks of 32-row tiles per wave, by the table's
 // width):
-//   32 x 9 queries over U{1024..8192} (16) 76.0 / 65.5 us, 32 x 32 (32) 140 / 118, 32 x 64 (64) 265 / 211;
-//   16/16 heads, 16 x 20 over U{2000..4000} (8) 59.5 / 53.1, 16 x 64 (16) 102 / 94;
-//   16/2 heads, 16 x 16 over U{2000..4000} (4) 38.1 / 47.8; 1 x 64 over 8000 (2) 28.4 / 33.4, 1 x 17 (1)
-//   22.9 / 24.4, 1 x 64 over 100 (less) 9.6 / 11.9.
-// An odd number of 16 rows leaves half a tile empty: 16/4 heads, 32 x 12 over U{500..4000} 40.3 / 45.4.
+//   32 x 9 queries over U{1024..8192} (16) 72.1 / 64.2 us, 32 x 32 (32) 132 / 114, 32 x 64 (64) 251 / 211;
+//   16/16 heads, 16 x 20 over U{2000..4000} (8) 55.1 / 49.7; 16/2 heads, 32 x 16 (8) 55.0 / 51.5; 4 x 64
+//   over 8000 (8) 58.4 / 54.1;
+//   4 x 32 over 8000 (4) 36.4 / 35.2; 16/2 heads, 16 x 16 over U{2000..4000} (4) 36.1 / 37.2; 1 x 64 over
+//   8000 (2) 24.1 / 27.7, 16/2 heads, 8 x 16 over 2000 (1) 19.5 / 21.6, 1 x 64 over 100 (less) 9.4 / 12.0.
+// An odd number of 16 rows leaves half a tile empty.
 bool wide_tiles(int64_t rows, int64_t chunks) {
   const int64_t tiles = (rows + 2 * kR - 1) / (2 * kR);
   return rows > kR && (rows - 1) / kR % 2 == 1 && tiles <= INT32_MAX / (chunks < 1 ? 1 : chunks) &&
@@ -879,11 +883,11 @@ bool plan_of(int batch, int max_queries, int num_q_heads, int num_kv_heads, int 
 // CU 4 us longer than one, and more CUs then share a group's keys in less: unless there are groups for
 // many of them, or the second kernel, 3 us of the host's time, is what a call waits for.
 // Measured, graph replays, cut between waves / a workgroup each, 16/8 heads of 128:
-//   1 x 100 keys 7.8 / 6.0 us, 1 x 1000 8.7 / 7.7, 4 x 1024 9.4 / 8.5, 32 x U{100..1000} 14.3 / 10.1;
-//   1 x 1280 8.7 / 10.6, 1 x 2048 9.2 / 12.0, 4 x 2048 10.1 / 12.5 (called one by one: 16.3 / 13.6), 8 x
-//   2048 12.5 / 12.8, 12 x 2048 14.8 / 13.2, 32 x 2048 21.3 / 17.8;
-//   32 x U{100..4096} 23.7 / 23.6, 32 x 4096 33.5 / 30.0;
-//   33 x U{100..256} (264 groups) 9.2 / 10.3, 64 x U{100..300} 11.9 / 14.6.
+//   1 x 100 keys 7.1 / 5.9 us, 1 x 1000 8.6 / 7.6, 4 x 1024 9.3 / 8.2, 32 x U{100..1000} 13.9 / 9.5;
+//   1 x 1280 8.7 / 11.0, 1 x 2048 9.0 / 12.0, 4 x 2048 9.7 / 12.2 (called one by one: 15.7 / 12.7), 8 x
+//   2048 11.8 / 12.5, 12 x 2048 13.7 / 12.9, 16 x U{100..2048} 14.4 / 12.9, 32 x 2048 20.4 / 16.9;
+//   32 x U{100..4096} 23.4 / 23.2, 32 x 4096 32.2 / 29.0;
+//   33 x U{100..256} (264 groups) 9.5 / 10.1, 64 x U{100..300} 11.6 / 14.2, 128 x 1024 31.2 / 36.6.
 constexpr int kWholeWaves = 16;
 constexpr int64_t kWholeGroups = 256, kWholeKeys = 1024, kWholeMinGroups = 32;
 bool whole_groups(int rows, int head_dim, int64_t groups, int64_t max_keys) {
@@ -923,13 +927,14 @@ int launch(const AttnArgs& a, hipStream_t s) {
   if (st != NVK_OK) return st;
   const dim3 mgrid(a.max_tiles * ((a.rec_rows + 1) / 2), a.num_kv_heads, a.batch);
   // By the parts that a group has on average, where it has any: a wave fetches 4 in a round trip.
-  // 64 x U{100..2048} keys, 16/8 heads (4 parts): 24.4 us with one wave per row pair, 23.1 with four; 32
-  // x 6 over U{1024..8192} (8 parts): 42.7 with one, 42.1 with four or sixteen.
+  // One wave / four per row pair, 16/8 heads: 16/2 heads, 8 x 16 queries over 2000 (4 parts) 18.3 / 18.9
+  // us; 8 x 1 over 4000 (8) 14.7 / 14.4, 4 over U{8192..32768} (16) 28.5 / 26.6; four / sixteen: 2 over
+  // 16000 (32) 15.3 / 15.4, 1 over 30000 (64) 16.3 / 15.2, 8/1 heads, 1 over 100000 (512) 27.4 / 19.7.
   const int64_t parts =
       a.n_waves / kWavesPerWG / ((int64_t)a.batch * a.num_kv_heads * a.max_tiles);
-  if (parts >= 16)
+  if (parts >= 32)
     hipLaunchKernelGGL((fp4_merge_kernel<HD, F16, 16>), mgrid, dim3(64 * 16), 0, s, a);
-  else if (parts >= 4)
+  else if (parts >= 8)
     hipLaunchKernelGGL((fp4_merge_kernel<HD, F16, 4>), mgrid, dim3(64 * 4), 0, s, a);
   else
     hipLaunchKernelGGL((fp4_merge_kernel<HD, F16, 1>), mgrid, dim3(64), 0, s, a);
