@@ -303,18 +303,28 @@ __global__ __launch_bounds__(64 * W, W == kWavesPerWG ? 2 : 1) void fp4_attentio
   auto locate = [&](int keys, int ss, int hh, int kk) {
     Where p;
     const const_i32* bt = (const_i32*)(a.block_tables + (int64_t)ss * a.bt_stride);
+    // the blocks' pages and places first, so that the loads of the page ids go out together
+    const int key0 = kk * kCK;
+    int logical = a.bs_shift >= 0 ? key0 >> a.bs_shift : key0 / a.block_size;
+    int off = key0 - logical * a.block_size;
+    int page[kBlk], offs[kBlk];
+    p.in_page = off;
+    page[0] = bt[logical];
+    offs[0] = off;
+#pragma unroll
+    for (int b = 1; b < kBlk; ++b) {  // a block past the keys: the last one, nothing of it counts
+      const bool more = key0 + 16 * b < keys, next = off + 16 == a.block_size;
+      logical += more && next;
+      off = !more ? off : next ? 0 : off + 16;
+      page[b] = bt[logical];
+      offs[b] = off;
+    }
 #pragma unroll
     for (int b = 0; b < kBlk; ++b) {
-      int key = kk * kCK + 16 * b;
-      if (key >= keys) key = kk * kCK;  // a block past the keys: any block, nothing of it counts
-      const int logical = a.bs_shift >= 0 ? key >> a.bs_shift : key / a.block_size;
-      int page = bt[logical];
-      if (page < 0 || page >= a.num_blocks) page = 0;
-      const int off = key - logical * a.block_size;
-      const uint64_t head = (uint64_t)(uint32_t)page * page_bytes + (uint64_t)(uint32_t)hh * head_bytes;
-      p.row[b] = head + (uint32_t)off * RB;
-      p.scale[b] = (head >> 3) + (uint32_t)off * 2;  // 2 bytes of scale per 16 of codes
-      p.in_page = off;
+      const int pg = page[b] < 0 || page[b] >= a.num_blocks ? 0 : page[b];
+      const uint64_t head = (uint64_t)(uint32_t)pg * page_bytes + (uint64_t)(uint32_t)hh * head_bytes;
+      p.row[b] = head + (uint32_t)offs[b] * RB;
+      p.scale[b] = (head >> 3) + (uint32_t)offs[b] * 2;  // 2 bytes of scale per 16 of codes
     }
     return p;
   };
@@ -328,9 +338,16 @@ __global__ __launch_bounds__(64 * W, W == kWavesPerWG ? 2 : 1) void fp4_attentio
     }
     return locate(keys, ss, hh, kk);
   };
-  auto pick = [](const uint64_t* v, int i) {  // v[i] of a lane's block i
-    if constexpr (kBlk == 1) return v[0];
-    else return i & 2 ? (i & 1 ? v[3] : v[2]) : (i & 1 ? v[1] : v[0]);
+  // v[i] of a lane's block i.  (All four read first: a choice between their addresses would put them in
+  // scratch memory.)
+  auto pick = [](const uint64_t (&v)[kBlk], int i) {
+    if constexpr (kBlk == 1) {
+      return v[0];
+    } else {
+      const uint64_t v0 = v[0], v1 = v[1], v2 = v[2], v3 = v[3];
+      const uint64_t lo = i & 1 ? v1 : v0, hi = i & 1 ? v3 : v2;
+      return i & 2 ? hi : lo;
+    }
   };
   auto issue_keys = [&](const Where& p, kvec (&kraw)[4]) {
     const uint8_t* kp = a.k_data + (kBlk == 1 ? p.row[0] : pick(p.row, r >> 2)) + k_off;
