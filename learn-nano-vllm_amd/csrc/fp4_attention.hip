@@ -855,10 +855,12 @@ struct Plan {
 //   over 8000 (8) 58.4 / 54.1;
 //   4 x 32 over 8000 (4) 36.4 / 35.2; 16/2 heads, 16 x 16 over U{2000..4000} (4) 36.1 / 37.2; 1 x 64 over
 //   8000 (2) 24.1 / 27.7, 16/2 heads, 8 x 16 over 2000 (1) 19.5 / 21.6, 1 x 64 over 100 (less) 9.4 / 12.0.
-// An odd number of 16 rows leaves half a tile empty.
+// An odd number of 16-row blocks leaves half a tile empty, which 7 are enough to make up for (64 x 100
+// queries, 13 blocks, 206 / 170; 32 x 12, 16/4 heads, 3 blocks, over U{500..4000} 37.6 / 37.5; 5 blocks: 32
+// x 20, 16/4 heads, 51.9 / 53.9, 32 x 40 160 / 158).
 bool wide_tiles(int64_t rows, int64_t chunks) {
-  const int64_t tiles = (rows + 2 * kR - 1) / (2 * kR);
-  return rows > kR && (rows - 1) / kR % 2 == 1 && tiles <= INT32_MAX / (chunks < 1 ? 1 : chunks) &&
+  const int64_t blocks = (rows + kR - 1) / kR, tiles = (blocks + 1) / 2;
+  return (blocks % 2 == 0 || blocks >= 7) && tiles <= INT32_MAX / (chunks < 1 ? 1 : chunks) &&
          tiles * chunks >= 6 * kMaxWGs * kWavesPerWG;
 }
 
@@ -959,11 +961,12 @@ int launch(const AttnArgs& a, hipStream_t s) {
 }
 
 // Long query ranges go through f16 pages (fp4.h).
-// From 129 rows (queries x G) per kv head on.  Measured, the kernel above / pages, 16/8 heads:
-//   128 rows: 32 x 64 queries over U{1024..8192} 210 / 348 us, 1 x 64 over 8000 29 / 37, 4 x 64 over 300
-//   18.5 / 18.6; 192: 398 / 428 (tiles of 16 rows), 35.6 / 36.5, 22.3 / 18.6; 256: 524 / 434, 41.5 / 36.9,
-//   16/4 heads, 8 x 64 over 2000 43.5 / 36.2, 16/16 heads, 16 x 192 (192 rows) 279 / 254.
-constexpr int kDirectRows = 128;
+// From 193 rows (queries x G) per kv head on.  Measured, the kernel above / pages, 16/8 heads:
+//   128 rows: 32 x 64 queries over U{1024..8192} 194 / 345 us, 1 x 64 over 8000 23.5 / 36.3, 4 x 64 over 300
+//   16.3 / 18.6; 192: 281 / 421, 29.4 / 35.9, 17.9 / 18.7, 16/16 heads, 16 x 192 over U{2000..4000} 201 /
+//   254; 200: 64 x 100 over U{600..1500} 170 / 184, 16 x 100 63 / 58; 240: 32 x 120 110 / 88; 256: 32 x 128
+//   over U{1024..8192} 371 / 424, over 256 43 / 36; 384: 565 / 557, 1 x 192 over 8000 43.4 / 41.2.
+constexpr int kDirectRows = 192;
 constexpr int64_t kPageBytesMost = (int64_t)512 << 20;  // pages of a part of the batch (one sequence: any)
 
 // Workspace of that route, for `part` sequences at a time.

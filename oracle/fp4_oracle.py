@@ -75,7 +75,7 @@ def store(rows, data, scale, slots, keys):
 
 def through_pages(n, g, d):
     """Whether n queries of g heads per kv head run over f16 pages of the keys and values."""
-    return n * g > 128 and d == 128 and g in (1, 2, 4, 8)
+    return n * g > 192 and d == 128 and g in (1, 2, 4, 8)
 
 
 def attention(q, k, v, n_keys, scale, pages=False):

@@ -106,7 +106,8 @@ def test_ragged_queries(news, cached, bs, dtype):
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
 @pytest.mark.parametrize("n,hq,hkv,d,bs", [(9, 16, 8, 128, 64), (16, 16, 8, 128, 16),
                                            (60, 16, 8, 128, 256), (30, 8, 8, 64, 64),
-                                           (4, 64, 8, 64, 16), (25, 8, 8, 128, 48)])
+                                           (4, 64, 8, 64, 16), (25, 8, 8, 128, 48),
+                                           (50, 16, 8, 128, 64)])
 def test_tiles_of_32_rows(n, hq, hkv, d, bs, dtype):
     """Tables that could hold 32768 tokens of each sequence: many chunks for every wave, by which tiles
     of 32 rows are chosen, over contexts that end anywhere."""
@@ -144,7 +145,7 @@ def test_one_workgroup_per_group_and_ranges_of_waves_agree(hq, hkv, d, bs, dtype
 def test_chunks_of_many_queries(hq, hkv, bs, dtype):
     """Over f16 pages (three heads per kv head: without), with chunks that end inside a tile, in front
     of everything, and sequences without queries or with fewer keys than queries."""
-    news, cached = [150, 33, 0, 64, 40], [300, 0, 20, 65, -10]
+    news, cached = [200, 33, 0, 64, 40], [300, 0, 20, 65, -10]
     lens = [a + b for a, b in zip(news, cached)]
     tables, nb = tables_of(lens, bs, 8)
     pages = Pages(12, nb, bs, hkv, 128, dtype)
@@ -161,21 +162,21 @@ def test_chunks_of_many_queries(hq, hkv, bs, dtype):
 @pytest.mark.parametrize("up", [2.0 ** 20, 2.0 ** -20])
 def test_chunks_of_queries_far_from_one(up):
     """bf16 queries outside f16's range, and values that only an eighth of fits it."""
-    hq, hkv, n = 2, 1, 70
-    tables, nb = tables_of([90], 64, 8)
+    hq, hkv, n = 2, 1, 100
+    tables, nb = tables_of([120], 64, 8)
     pages = Pages(12, nb, 64, hkv, 128)
     big = rng_rows(3, (nb * 64, hkv, 128), "bf16").double().numpy() * 2.0 ** 16
     orc.store(big, *pages.np[1], np.arange(nb * 64), False)
     q = (rng_rows(13, (n, hq, 128), "bf16") * up).cuda()
     scale = 128 ** -0.5 / up
-    out = flash_attn_with_kvcache(q[None], *pages.gpu(), cache_seqlens=_int([90]),
+    out = flash_attn_with_kvcache(q[None], *pages.gpu(), cache_seqlens=_int([120]),
                                   block_table=_int(tables), softmax_scale=scale, causal=True)
-    ref, size = _reference(q, pages, tables, [n], [90], scale)
+    ref, size = _reference(q, pages, tables, [n], [120], scale)
     assert_close(out[0], ref, size, "bf16", "fp4 far queries")
 
 
 def test_chunks_do_not_see_what_is_not_finite_behind_the_mask():
-    n, lens = 70, [100]
+    n, lens = 100, [130]
     tables, nb = tables_of(lens, 64, 4)
     pages = Pages(7, nb, 64, 2, 128)
     q = rng_rows(1, (n, 4, 128), "bf16").cuda()
@@ -184,14 +185,14 @@ def test_chunks_do_not_see_what_is_not_finite_behind_the_mask():
         pages.np[i][1][tables[0][1], i, 2, 90 - 64] = np.nan
     out = flash_attn_with_kvcache(q[None], *pages.gpu(), cache_seqlens=_int(lens),
                                   block_table=_int(tables), causal=True)[0]
-    sees = 90 - (100 - n)                             # the first query that sees it
+    sees = 90 - (130 - n)                             # the first query that sees it
     assert torch.isnan(out[sees:]).all()
     assert_close(out[:sees], ref[:sees], size[:sees], "bf16", "fp4 chunk, masked NaN")
 
 
 def test_a_batch_larger_than_the_pages_goes_in_parts():
     """Tables of 16384 tokens: 64 MiB of f16 keys and values for a sequence, so 8 at a time."""
-    lens, n = [40, 300, 17, 90, 33, 50, 64, 65, 129, 200, 35], 70
+    lens, n = [40, 300, 17, 90, 33, 50, 64, 65, 129, 200, 35], 100
     tables, nb = tables_of(lens, 256, 4)
     pages = Pages(7, nb, 256, 8, 128)
     wide = np.full((len(lens), 64), -1, np.int32)
@@ -205,8 +206,8 @@ def test_a_batch_larger_than_the_pages_goes_in_parts():
 
 
 def test_a_captured_chunk_follows_its_inputs():
-    lens, n = [100, 160], 70
-    tables, nb = tables_of([160] * 2, 64, 3)
+    lens, n = [130, 190], 100
+    tables, nb = tables_of([190] * 2, 64, 3)
     pages = Pages(7, nb, 64, 2, 128)
     q, keys = rng_rows(1, (2, n, 4, 128), "bf16").cuda(), _int(lens)
     call = lambda: flash_attn_with_kvcache(q, *gpu, cache_seqlens=keys, block_table=bt, causal=True)
@@ -216,7 +217,7 @@ def test_a_captured_chunk_follows_its_inputs():
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         out = call()
-    for i, now in enumerate([lens, [60, 71], [160, 160], lens]):
+    for i, now in enumerate([lens, [90, 101], [190, 190], lens]):
         q.copy_(rng_rows(20 + i, (2, n, 4, 128), "bf16"))
         keys.copy_(_int(now))
         graph.replay()

@@ -114,7 +114,7 @@ def test_a_layer_over_4_bit_caches():
         m.check_caches()
 
         # the next chunk of each, over what the caches hold; the module called by itself
-        for news in ([90, 1, 20], [3, 8, 1]):           # through f16 pages, and not
+        for news in ([100, 1, 20], [3, 8, 1]):           # through f16 pages, and not
             lens = [a + b for a, b in zip(lens, news)]
             slots, pos = _prefill_context(news, lens, True)
             qkv = m.qkv(sum(news))
