@@ -14,9 +14,23 @@
 // 2, 4 and 8 rows per thread: stored in 18.9 / 20.7 / 23.1 us, and 4096 tokens in 8.0 / 8.7 / 9.6
 // against 7.0.  The codes are read with plain loads: non-temporal ones take 5 % less time where the
 // codes come from HBM (35000 tokens 40.9 / 43.0 us), 30 % more where they were just written.
+// Non-temporal stores of the rows end the read-back sooner and make whoever reads them later: 35000
+// tokens 34 us against 42, with a reader behind it 91.3 against 90.2; 8300 tokens 9.5 against 12.3, and
+// 28.1 against 26.1.
 #include "fp4.h"
 
 namespace {
+
+// Grids: heads, pieces of the tokens, and beyond kGridY pieces more of those along z.  Heads first: the
+// workgroups of one piece, which share its rows on the 16-bit side, run side by side, and (8 heads) a
+// head stays on one of the 8 XCDs, each with an L2 of its own: 16 tokens' scales are a quarter of a
+// line.  Pieces first: 16384 tokens stored and read back 34.1 us, not 31.9; 38176 read back 45.0, not
+// 43.9; with four neighbouring pieces to one XCD 32.5 and 46.6.
+constexpr int kGridY = 32768;
+dim3 heads_first(int heads, int64_t pieces) {
+  return dim3(heads, (unsigned)(pieces < kGridY ? pieces : kGridY),
+              (unsigned)((pieces + kGridY - 1) / kGridY));
+}
 
 struct CacheArgs {
   uint8_t *k_data, *v_data;
@@ -88,8 +102,8 @@ __global__ __launch_bounds__(256) void fp4_store_kernel(CacheArgs a, const uint1
                                                         int64_t value_stride) {
   constexpr int kLanes = HD / 8, kRows = 256 / kLanes;  // lanes of a row, rows of a workgroup
   const int u = threadIdx.x % kLanes;
-  const int h = blockIdx.y;
-  const int64_t t = (int64_t)blockIdx.x * kRows + threadIdx.x / kLanes;
+  const int h = blockIdx.x;
+  const int64_t t = ((int64_t)blockIdx.z * kGridY + blockIdx.y) * kRows + threadIdx.x / kLanes;
   if (t >= a.n_tokens) return;  // whole rows: the lanes of a group leave together
   const int64_t col = (int64_t)h * HD + 8 * u;
   const int slot = a.slots[t];  // the rows are loaded whatever it is: they do not wait for it
@@ -128,8 +142,8 @@ __global__ __launch_bounds__(256) void fp4_load_kernel(CacheArgs a, uint16_t* ke
                                                        int64_t value_stride) {
   constexpr int kLanes = HD / 8, kRows = 256 / kLanes;
   const int u = threadIdx.x % kLanes;
-  const int h = blockIdx.y;
-  const int64_t t = (int64_t)blockIdx.x * kRows + threadIdx.x / kLanes;
+  const int h = blockIdx.x;
+  const int64_t t = ((int64_t)blockIdx.z * kGridY + blockIdx.y) * kRows + threadIdx.x / kLanes;
   if (t >= a.n_tokens) return;
   const int slot = a.slots[t];
   nvk_u32x4 k = {0u, 0u, 0u, 0u}, v = k;
@@ -171,22 +185,24 @@ __device__ void uniform_prefix(const Fp4Expand& a) {
   }
 }
 
-// Keys and values of each sequence's pages as f16 (see Fp4Expand).  grid = (16-token pieces of a
-// sequence, sequences, pairs of heads); 16 lanes a row.  32 sequences of U{612..1536} tokens and 8 heads,
+// Keys and values of each sequence's pages as f16 (see Fp4Expand).  grid = (pairs of heads, 16-token
+// pieces of a sequence, sequences); 16 lanes a row.  32 sequences of U{612..1536} tokens and 8 heads,
 // 31 MB read and 110 written: 39 us; with all heads of a piece in a workgroup 41, with one head 48, and
 // other mappings (a quad per row, 4 heads of a token per wave, loads a step ahead) 41 to 48.
 template <bool F16>
 __global__ __launch_bounds__(256) void fp4_expand_kernel(Fp4Expand a) {
   constexpr int HD = 128, HB = 2;
-  const int s = blockIdx.y, h0 = HB * blockIdx.z;
-  if (blockIdx.x == 0 && h0 == 0) {
+  const int folds = (a.pages_per_seq * (kFp4Page / 16) + kGridY - 1) / kGridY;
+  const int s = folds == 1 ? blockIdx.z : blockIdx.z / folds;
+  const int piece = (blockIdx.z - s * folds) * kGridY + blockIdx.y, h0 = HB * blockIdx.x;
+  if (piece == 0 && h0 == 0) {
     for (int i = threadIdx.x; i < a.pages_per_seq; i += 256)
       a.tables[(int64_t)s * a.pages_per_seq + i] = s * a.pages_per_seq + i;
     if (a.cu_q_out && s == 0) uniform_prefix(a);
   }
   // the page is looked up beside the length, not after it
   const int u = threadIdx.x % 16;
-  const int p = blockIdx.x * 16 + threadIdx.x / 16;
+  const int p = piece * 16 + threadIdx.x / 16;
   const int logical = a.bs_shift >= 0 ? p >> a.bs_shift : p / a.block_size;
   int page = a.block_tables[s * a.bt_stride + min(logical, a.max_blocks - 1)];
   int64_t keys = a.lens ? a.lens[a.first + s] : (int64_t)a.cu_k[s + 1] - a.cu_k[s];
@@ -298,7 +314,7 @@ struct StoreLaunch {
   template <int HD, bool F16>
   int operator()() const {
     constexpr int kRows = 256 / (HD / 8);
-    const dim3 grid((unsigned)((a.n_tokens + kRows - 1) / kRows), a.num_kv_heads);
+    const dim3 grid = heads_first(a.num_kv_heads, (a.n_tokens + kRows - 1) / kRows);
     hipLaunchKernelGGL((fp4_store_kernel<HD, F16>), grid, dim3(256), 0, s, a, k, ks, v, vs);
     return nvk_launch_status();
   }
@@ -312,7 +328,7 @@ struct LoadLaunch {
   template <int HD, bool F16>
   int operator()() const {
     constexpr int kRows = 256 / (HD / 8);
-    const dim3 grid((unsigned)((a.n_tokens + kRows - 1) / kRows), a.num_kv_heads);
+    const dim3 grid = heads_first(a.num_kv_heads, (a.n_tokens + kRows - 1) / kRows);
     hipLaunchKernelGGL((fp4_load_kernel<HD, F16>), grid, dim3(256), 0, s, a, k, ks, v, vs);
     return nvk_launch_status();
   }
@@ -321,7 +337,8 @@ struct LoadLaunch {
 }  // namespace
 
 int fp4_expand_launch(const Fp4Expand& p, hipStream_t stream) {
-  const dim3 grid(p.pages_per_seq * (kFp4Page / 16), p.batch, (p.num_kv_heads + 1) / 2);
+  dim3 grid = heads_first((p.num_kv_heads + 1) / 2, (int64_t)p.pages_per_seq * (kFp4Page / 16));
+  grid.z *= p.batch;
   if (p.f16)
     hipLaunchKernelGGL(fp4_expand_kernel<true>, grid, dim3(256), 0, stream, p);
   else

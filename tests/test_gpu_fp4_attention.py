@@ -6,8 +6,8 @@ import torch
 
 from fp4_utils import DTYPES, Pages, assert_close, rng_rows, tables_of
 from gpu_utils import say
-from nanovllm_amd import (Fp4Cache, flash_attn_varlen_func, flash_attn_with_kvcache, paged_decode,
-                          varlen_prefill)
+from nanovllm_amd import (Fp4Cache, flash_attn_varlen_func, flash_attn_with_kvcache, load_kvcache,
+                          paged_decode, store_kvcache, varlen_prefill)
 from oracle import fp4_oracle as orc
 
 pytestmark = pytest.mark.gpu
@@ -203,6 +203,28 @@ def test_a_batch_larger_than_the_pages_goes_in_parts():
                                   causal=True)
     ref, size = _reference(q.flatten(0, 1), pages, tables, [n] * len(lens), lens, 128 ** -0.5)
     assert_close(out, ref, size, "bf16", "fp4 parts of a batch")
+
+
+def test_a_chunk_over_more_keys_than_one_grid_dimension_holds():
+    """More than 32768 pieces of 16 keys.  Query i's key, 30 / |q| times the query, is the only one with
+    weight: scores of 25 and more against N(0, 1), so the others weigh 525288 e^(0.5 - 25), 1e-5."""
+    n, keys, d, bs = 200, 16 * 32768 + 1000, 128, 256
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    rand = lambda *shape: torch.randn(shape, generator=gen, device="cuda")
+    q = rand(n, 1, d).to(torch.bfloat16)
+    at = torch.arange(n, device="cuda") * 4 + keys - 1000 - 100     # both sides of key 524288
+    k, v = (rand(keys, 1, d).to(torch.bfloat16) for _ in range(2))
+    k[at] = (30 * q / q.float().norm(dim=-1, keepdim=True)).to(torch.bfloat16)
+    caches = [Fp4Cache.zeros(-(-keys // bs), bs, 1, d) for _ in range(2)]
+    slots = torch.arange(keys, dtype=torch.int32, device="cuda")
+    store_kvcache(k, v, *caches, slots)
+    say("fp4 chunk over 525288 keys")
+    out = flash_attn_with_kvcache(q[None], *caches, cache_seqlens=_int([keys]), causal=True,
+                                  block_table=_int(np.arange(-(-keys // bs))[None]))[0]
+    want = load_kvcache(*caches, slots[at], torch.float16)[1].float()
+    # the output's rounding, three of f16 (page, probability, the values compared with), the others
+    bound = (2.0 ** -8 + 3 * 2.0 ** -11) * want.abs() + 1e-4
+    assert ((out.float() - want).abs() <= bound).all()
 
 
 def test_a_captured_chunk_follows_its_inputs():

@@ -151,3 +151,23 @@ def test_offsets_past_32_bits():
             * scale.astype(np.float64).repeat(32, -1)
         assert torch.equal(got.cpu(), torch.from_numpy(want).float().to(torch.bfloat16))
     assert int(kc.data[1:nb - 8].count_nonzero()) == 0
+
+
+def test_more_tokens_than_one_grid_dimension_holds():
+    """More than 32768 pieces of 16 tokens: the same as two calls of fewer."""
+    n, d, bs = 16 * 32768 + 1000, 128, 256
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    key, value = torch.randn(2, n, 1, d, generator=gen, device="cuda").to(torch.bfloat16)
+    slots = torch.arange(n, dtype=torch.int32, device="cuda").flip(0)
+    once, twice = ([Fp4Cache.zeros(-(-n // bs), bs, 1, d) for _ in range(2)] for _ in range(2))
+    say("fp4 store and load of 525288 tokens")
+    store_kvcache(key, value, *once, slots)
+    half = n // 2
+    for part in (slice(0, half), slice(half, n)):
+        store_kvcache(key[part], value[part], *twice, slots[part])
+    rows = load_kvcache(*once, slots)
+    for i in range(2):
+        assert torch.equal(once[i].data, twice[i].data)
+        assert torch.equal(once[i].scale, twice[i].scale)
+        parts = [load_kvcache(*once, slots[part])[i] for part in (slice(0, half), slice(half, n))]
+        assert torch.equal(rows[i], torch.cat(parts))
