@@ -585,7 +585,8 @@ int nvk_fp4_load(const void* k_data, const void* k_scale, const void* v_data, co
  * Query i of Lq sees key j iff j <= i + Lk - Lq; one that sees none is written as zeros.
  * q, out, block_tables, scale: as in nvk_paged_decode.  A page id outside [0, num_blocks) is never
  *   followed; the output of a sequence that names one is unspecified.
- * Up to 192 rows (queries x G): the scores are f32 sums of exact products; a probability times its
+ * Up to 192 rows (queries x G), and for steps of less than 16384 chunks (64 keys under 16 rows of
+ *   a kv head, by the call's bounds): the scores are f32 sums of exact products; a probability times its
  *   value's scale is rounded to f16 before the product with the codes, whose sums are f32.
  *   More rows, head_dim 128 and G 1, 2, 4 or 8: keys and values pass through f16 pages in the
  *   workspace (512 MiB of them, or one sequence's if that is more; a larger batch goes in parts),

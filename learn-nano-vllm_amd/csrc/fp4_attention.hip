@@ -12,7 +12,7 @@
 //     contiguous ranges, one per wave.  The waves of a workgroup join a group that is cut between
 //     them in LDS; one cut between workgroups leaves (O, m, l) records that a second kernel merges.
 //     (Records of every wave: 192 x U{256..4096} keys, 16/2 heads, 34.1 us and not 31.6, 8 x 16 queries
-//     over 2000 27.1 and not 19.1.)  A few short groups of a few rows get a workgroup of 16 waves each.
+//     over 2000 27.1 and not 19.1.)  Short groups get a workgroup of 4 or 8 waves each.
 //   * S^T = K Q^T on v_mfma_f32_16x16x32: operand row m = 4 a + i of key block b is key
 //     16 a + 4 b + i of the chunk, so lane (g, r) ends up with the scores of keys 16 g .. +15 of
 //     row r in order: the order in which ds_read_b64_tr_b4 hands it the values of a dimension.
@@ -198,11 +198,13 @@ struct KeyVec<64> {
 // A score is then NG / NC products with scales in each of NC lanes, which add up, instead of NG in
 // one; and a lane needs P vs for its own groups only, whose dimensions alone are kept of its output.
 // NT: 16-row blocks of a tile.  Two share what the wave loads and converts (see wide_tiles).
-// W waves per workgroup.  WHOLE: a workgroup owns one group, its waves an equal part of the chunks
-// each; they join their states in LDS, and nothing is left to a second kernel.
+// W waves per workgroup.  WHOLE: a workgroup owns one group (grid = kv heads, sequences, tiles), its
+// waves an equal part of the chunks each; they join their states in LDS, and nothing is left to a
+// second kernel (see whole_waves).  Waves per SIMD: as many as the registers allow.
 template <int HD, bool F16, bool ONEPAGE, int NC, int NT = 1, int W = kWavesPerWG,
           bool WHOLE = false>
-__global__ __launch_bounds__(64 * W, W == kWavesPerWG ? 2 : 1) void fp4_attention_kernel(AttnArgs a) {
+__global__ __launch_bounds__(64 * W, WHOLE ? (NC >= 4 || HD == 64 ? 4 : NC == 2 && W == 4 ? 3 : 2)
+                                           : 2) void fp4_attention_kernel(AttnArgs a) {
   using E = NvkElt<F16>;
   typedef typename E::vec8 vec8;
   typedef typename KeyVec<HD>::type kvec;
@@ -213,7 +215,8 @@ __global__ __launch_bounds__(64 * W, W == kWavesPerWG ? 2 : 1) void fp4_attentio
   constexpr int kBlk = ONEPAGE ? 1 : 4;    // pages looked up per chunk
   constexpr int kRec = HD + 4;
   constexpr int NS = NG / NC;              // groups of a column
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[W * kBuf];
+  constexpr int kState = WHOLE ? kR / NC * kRec * (int)sizeof(float) : 0;  // of a wave's rows, at the end
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[W * (kState > kBuf ? kState : kBuf)];
   __shared__ int s_cs[WHOLE ? 1 : kMaxBatch + 1];
   __shared__ int s_wsum[kWavesPerWG];
   // !WHOLE: what waves 1 .. W - 1 hold of a group that began before them: O, (m, l), whether it ended there
@@ -233,11 +236,11 @@ __global__ __launch_bounds__(64 * W, W == kWavesPerWG ? 2 : 1) void fp4_attentio
   if constexpr (WHOLE) {
     kvh = blockIdx.x;
     s = blockIdx.y;
-    tile = 0;
+    tile = blockIdx.z;
     sq = seq_of(a, s);
     n = uniform(chunks_of(sq));
     tiles = 1;
-    if (sq.queries <= 0) return;
+    if (sq.queries * a.G <= tile * kR) return;
     c0 = n * wave / W;
     c1 = n * (wave + 1) / W;
     k = c0;
@@ -696,7 +699,7 @@ __global__ __launch_bounds__(64 * W, W == kWavesPerWG ? 2 : 1) void fp4_attentio
   } else {
     // Wave v's rows to LDS (the values' buffers, used up): O, m, l; then a thread sums 4 dimensions of
     // a row over the waves.
-    static_assert(NT == 1 && W * (kR / NC) * kRec * 4 <= W * kBuf, "the states fit the buffers");
+    static_assert(NT == 1, "rows of one block");
     float* st = reinterpret_cast<float*>(lds);
     const float l_tot = nvk_sum_xor32(sum_xor16(l_part[0][0] + l_part[0][1]));
     nvk_f32x4 o[kKeep];
@@ -704,7 +707,7 @@ __global__ __launch_bounds__(64 * W, W == kWavesPerWG ? 2 : 1) void fp4_attentio
     wait_reads();
     __syncthreads();
     if (row_valid[0]) {
-      float* rec = st + (wave * a.rec_rows + row) * kRec;
+      float* rec = st + (wave * (kR / NC) + row) * kRec;
 #pragma unroll
       for (int j = 0; j < kKeep; ++j) *reinterpret_cast<nvk_f32x4*>(rec + d0 + 16 * j) = o[j];
       if (g == 0 && g0 == 0) {
@@ -713,29 +716,31 @@ __global__ __launch_bounds__(64 * W, W == kWavesPerWG ? 2 : 1) void fp4_attentio
       }
     }
     __syncthreads();
-    const int mrow = tid / (HD / 4), d = 4 * (tid % (HD / 4));
-    if (mrow >= sq.queries * a.G || mrow >= a.rec_rows) return;
-    float M = -INFINITY;
+    const int d = 4 * (tid % (HD / 4)), rows = min(sq.queries * a.G - tile * kR, kR / NC);
+    for (int mrow = tid / (HD / 4); mrow < rows; mrow += 64 * W / (HD / 4)) {
+      float M = -INFINITY;
 #pragma unroll
-    for (int v = 0; v < W; ++v) M = fmaxf(M, st[(v * a.rec_rows + mrow) * kRec + HD]);
-    const float mref = M == -INFINITY ? 0.f : M;
-    float L = 0.f;
-    nvk_f32x4 O = {0.f, 0.f, 0.f, 0.f};
+      for (int v = 0; v < W; ++v) M = fmaxf(M, st[(v * (kR / NC) + mrow) * kRec + HD]);
+      const float mref = M == -INFINITY ? 0.f : M;
+      float L = 0.f;
+      nvk_f32x4 O = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int v = 0; v < W; ++v) {
-      const float* rec = st + (v * a.rec_rows + mrow) * kRec;
-      const float wt = nvk_fast_exp2(rec[HD] - mref);
-      L += rec[HD + 1] * wt;
-      O += wt * *reinterpret_cast<const nvk_f32x4*>(rec + d);
+      for (int v = 0; v < W; ++v) {
+        const float* rec = st + (v * (kR / NC) + mrow) * kRec;
+        const float wt = nvk_fast_exp2(rec[HD] - mref);
+        L += rec[HD + 1] * wt;
+        O += wt * *reinterpret_cast<const nvk_f32x4*>(rec + d);
+      }
+      const float inv = L == 0.f ? 0.f : 1.f / L;
+      const int rr = tile * kR + mrow;
+      const int mt = a.G == 1 ? rr : (int)__umulhi((uint32_t)rr, a.g_inverse);
+      nvk_u32x2 wv;
+      wv.x = E::pack2(O[0] * inv, O[1] * inv);
+      wv.y = E::pack2(O[2] * inv, O[3] * inv);
+      *reinterpret_cast<nvk_u32x2*>(a.out + (int64_t)(sq.row0 + mt) * a.out_stride_tok +
+                                    (int64_t)(kvh * a.G + rr - mt * a.G) * a.out_stride_head +
+                                    d) = wv;
     }
-    const float inv = L == 0.f ? 0.f : 1.f / L;
-    const int mt = a.G == 1 ? mrow : (int)__umulhi((uint32_t)mrow, a.g_inverse);
-    nvk_u32x2 wv;
-    wv.x = E::pack2(O[0] * inv, O[1] * inv);
-    wv.y = E::pack2(O[2] * inv, O[3] * inv);
-    *reinterpret_cast<nvk_u32x2*>(a.out + (int64_t)(sq.row0 + mt) * a.out_stride_tok +
-                                  (int64_t)(kvh * a.G + mrow - mt * a.G) * a.out_stride_head + d) =
-        wv;
   }
 }
 
@@ -897,35 +902,62 @@ bool plan_of(int batch, int max_queries, int num_q_heads, int num_kv_heads, int 
   return true;
 }
 
-// Whether a workgroup of 16 waves takes each group (WHOLE): one kernel less, for groups that are
-// few enough to have a CU each and short enough for one to stream.  Two chunks for a wave take a
-// CU 4 us longer than one, and more CUs then share a group's keys in less: unless there are groups for
-// many of them, or the second kernel, 3 us of the host's time, is what a call waits for.
-// Measured, graph replays, cut between waves / a workgroup each, 16/8 heads of 128:
-//   1 x 100 keys 7.1 / 5.9 us, 1 x 1000 8.6 / 7.6, 4 x 1024 9.3 / 8.2, 32 x U{100..1000} 13.9 / 9.5;
-//   1 x 1280 8.7 / 11.0, 1 x 2048 9.0 / 12.0, 4 x 2048 9.7 / 12.2 (called one by one: 15.7 / 12.7), 8 x
-//   2048 11.8 / 12.5, 12 x 2048 13.7 / 12.9, 16 x U{100..2048} 14.4 / 12.9, 32 x 2048 20.4 / 16.9;
-//   32 x U{100..4096} 23.4 / 23.2, 32 x 4096 32.2 / 29.0;
-//   33 x U{100..256} (264 groups) 9.5 / 10.1, 64 x U{100..300} 11.6 / 14.2, 128 x 1024 31.2 / 36.6.
-constexpr int kWholeWaves = 16;
-constexpr int64_t kWholeGroups = 256, kWholeKeys = 1024, kWholeMinGroups = 32;
-bool whole_groups(int rows, int head_dim, int64_t groups, int64_t max_keys) {
-  return rows <= kR / (head_dim / kFp4Group) && groups <= kWholeGroups &&
-         (max_keys <= kWholeKeys || (max_keys <= 2 * kWholeKeys && groups >= kWholeMinGroups));
+// Waves of a workgroup that takes a group by itself (WHOLE; 0: ranges): one kernel, no records, and all
+// of a group's chunks on their way at once, but a CU's time is that of the groups that fall to it.  By
+// the number of groups (a CU holds 2 to 4 such workgroups) and the most keys that one can have.  16/8
+// heads, ranges / 4 waves / 8 waves:
+//   up to 256 keys: 1 x 100 7.1 / 4.5 / 5.4 us, 64 x U{16..256} 11.1 / 7.3 / 7.9, 512 x U{16..256} 29.1 /
+//   23.0 / 38.5, 4 x 16 queries over 256 10.0 / 6.2 / 7.4, 64 x 96 over U{100..250} 57 / 50 / 127;
+//   up to 1024: 1 x 1000 8.4 / 8.5 / 7.5, 32 x U{100..1024} (256 groups) 13.9 / 11.0 / 9.8, 64 (512) 16.9 /
+//   14.2 / 14.4, 256 (2048) 37.5 / 34.8 / 37.3, 32 x 6 queries 19.2 / 13.2 / 11.9, 64 x 6 22.9 / 17.5 /
+//   20.5, 32 x 64 queries (2048) 47 / 42 / 66, 64 x 64 over U{600..1000} (4096) 88 / 93 / 149;
+//   up to 2048, ranges / 8 waves: 4 x 2048 (32) 9.7 / 12.4, but called one by one 15.7 / 12.7 (the second
+//   kernel is 3 us of the host's); 8 x 2048 (64) 11.8 / 12.5, 16 x U{100..2048} 14.6 / 13.1, 32 x 16.9 /
+//   14.3, 64 x 22.1 / 22.6, 64 x 2048 31.6 / 28.8, 128 x U{100..2048} (1024) 34.4 / 33.9; 6 queries: 32 x
+//   U{100..2048} 22.8 / 17.3, 64 x 29.3 / 31.0;
+//   up to 4096: 32 x U{100..4096} 23.4 / 23.1, 32 x 4096 32.8 / 29.3, 16 x 4096 (128) 20.1 / 23.0, 48 x
+//   U{100..4096} (384) 28.6 / 35.7; up to 8192: 32 x U{100..8192} 35.5 / 40.9.
+constexpr int kCUs = 256;
+int whole_waves(int rows, int head_dim, int64_t groups, int64_t max_keys) {
+  if (rows > 65535) return 0;  // tiles along a grid's z
+  if (max_keys <= 1024) {
+    if (groups * ((max_keys + kCK - 1) / kCK) >= 65536) return 0;
+    return max_keys > 256 && groups <= kCUs ? 8 : 4;
+  }
+  const bool few = rows <= kR / (head_dim / kFp4Group);
+  if (max_keys <= 2048) return groups >= kCUs / 8 && groups <= (few ? 4 : 1) * kCUs ? 8 : 0;
+  return max_keys <= 4096 && groups >= kCUs * 3 / 4 && groups <= kCUs ? 8 : 0;
 }
 
 template <int HD, bool F16>
-int launch(const AttnArgs& a, hipStream_t s) {
+int launch(const AttnArgs& a, int max_keys, hipStream_t s) {
   constexpr int NG = HD / kFp4Group;
   const dim3 grid(a.n_waves / kWavesPerWG), block(64 * kWavesPerWG);
-  const std::true_type yes;
-  const std::false_type no;
-  if (whole_groups(a.n_query * a.G, HD, (int64_t)a.batch * a.num_kv_heads, a.cap)) {
-    const auto one_kernel = [&](auto one) {
-      hipLaunchKernelGGL((fp4_attention_kernel<HD, F16, decltype(one)::value, NG, 1, kWholeWaves, true>),
-                         dim3(a.num_kv_heads, a.batch), dim3(64 * kWholeWaves), 0, s, a);
+  const int rows = a.n_query * a.G;
+  const std::integral_constant<int, 1> c1;
+  const std::integral_constant<int, 2> c2;
+  const std::integral_constant<int, NG> few;
+  const std::integral_constant<int, 4> four;
+  const std::integral_constant<int, 8> eight;
+  const int tiles16 = (rows + kR - 1) / kR;
+  if (const int w =
+          whole_waves(rows, HD, (int64_t)a.batch * a.num_kv_heads * tiles16, max_keys)) {
+    const auto one_kernel = [&](auto nc, auto waves) {
+      constexpr int NC = decltype(nc)::value, W = decltype(waves)::value;
+      const dim3 groups(a.num_kv_heads, a.batch, tiles16);
+      if (a.block_size % kCK)
+        hipLaunchKernelGGL((fp4_attention_kernel<HD, F16, false, NC, 1, W, true>), groups,
+                           dim3(64 * W), 0, s, a);
+      else
+        hipLaunchKernelGGL((fp4_attention_kernel<HD, F16, true, NC, 1, W, true>), groups,
+                           dim3(64 * W), 0, s, a);
     };
-    a.block_size % kCK ? one_kernel(no) : one_kernel(yes);
+    const auto by_rows = [&](auto waves) {
+      if (rows <= kR / NG) one_kernel(few, waves);
+      else if (rows <= kR / 2) one_kernel(c2, waves);
+      else one_kernel(c1, waves);
+    };
+    w == 4 ? by_rows(four) : by_rows(eight);
     return nvk_launch_status();
   }
   const auto main = [&](auto nc, auto nt) {
@@ -935,10 +967,7 @@ int launch(const AttnArgs& a, hipStream_t s) {
     else
       hipLaunchKernelGGL((fp4_attention_kernel<HD, F16, true, NC, NT>), grid, block, 0, s, a);
   };
-  const std::integral_constant<int, 1> c1;
-  const std::integral_constant<int, 2> c2;
-  const int rows = a.n_query * a.G;
-  if (rows <= kR / NG) main(std::integral_constant<int, NG>{}, c1);
+  if (rows <= kR / NG) main(few, c1);
   else if (rows <= kR / 2) main(c2, c1);
   else if (a.tile_rows == kR) main(c1, c1);
   else main(c1, c2);
@@ -961,12 +990,17 @@ int launch(const AttnArgs& a, hipStream_t s) {
 }
 
 // Long query ranges go through f16 pages (fp4.h).
-// From 193 rows (queries x G) per kv head on.  Measured, the kernel above / pages, 16/8 heads:
-//   128 rows: 32 x 64 queries over U{1024..8192} 194 / 345 us, 1 x 64 over 8000 23.5 / 36.3, 4 x 64 over 300
-//   16.3 / 18.6; 192: 281 / 421, 29.4 / 35.9, 17.9 / 18.7, 16/16 heads, 16 x 192 over U{2000..4000} 201 /
-//   254; 200: 64 x 100 over U{600..1500} 170 / 184, 16 x 100 63 / 58; 240: 32 x 120 110 / 88; 256: 32 x 128
-//   over U{1024..8192} 371 / 424, over 256 43 / 36; 384: 565 / 557, 1 x 192 over 8000 43.4 / 41.2.
+// From 193 rows (queries x G) per kv head on, where the step has work for more than that route's three
+// or four kernels: 16384 chunks of 64 keys under tiles of 16 rows.  Measured, the kernel above / pages,
+// 16/8 heads:
+//   128 rows: 32 x 64 queries over U{1024..8192} 194 / 345 us, 1 x 64 over 8000 23.5 / 36.3; 192: 281 / 421,
+//   29.4 / 35.9, 16/16 heads, 16 x 192 over U{2000..4000} 201 / 254; 200: 64 x 100 over U{600..1500} 170 /
+//   184, 16 x 100 63 / 58; 240: 32 x 120 110 / 88; 256: 32 x 128 over U{1024..8192} 371 / 424; 384: 565 / 557;
+//   by the chunks: 1 x 512 over 512 (4096) 11.7 / 19.9, 4 x 256 over 300 (5120) 15.8 / 19.1, 16 x 128 over
+//   256 (8192) 20.6 / 24.9, 8 x 200 over 500 (12800) 26.6 / 28.8, 1 x 1000 over 1000 (16000) 28.0 / 30.2,
+//   4 x 512 over 512 (16384) 30.4 / 24.7, 32 x 128 over 256 (16384) 37.5 / 33.8.
 constexpr int kDirectRows = 192;
+constexpr int64_t kDirectChunks = 16384;
 constexpr int64_t kPageBytesMost = (int64_t)512 << 20;  // pages of a part of the batch (one sequence: any)
 
 // Workspace of that route, for `part` sequences at a time.
@@ -982,6 +1016,9 @@ bool page_plan(int batch, int max_queries, int max_seqlen_k, int num_q_heads, in
     return false;
   int64_t keys = (int64_t)max_blocks * block_size;
   if (max_seqlen_k > 0 && max_seqlen_k < keys) keys = max_seqlen_k;
+  const int64_t tiles = ((int64_t)max_queries * G + kR - 1) / kR, chunks = (keys + kCK - 1) / kCK;
+  if (tiles * chunks < kDirectChunks && tiles * chunks * batch * num_kv_heads < kDirectChunks)
+    return false;
   if ((int64_t)num_kv_heads * head_dim >= (1 << 23) ||
       (int64_t)kFp4Page * num_kv_heads * head_dim * 2 > UINT32_MAX || num_kv_heads > 65535 ||
       (int64_t)max_queries * G > 65535 * (int64_t)128)
@@ -1170,6 +1207,8 @@ extern "C" int nvk_fp4_attention(const void* q, int64_t q_stride_tok, int64_t q_
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const bool f16 = dtype == NVK_DTYPE_F16;
   if (pages) return launch_pages(a, pp, num_q_heads, scale, f16, workspace, s);
-  if (head_dim == 128) return f16 ? launch<128, true>(a, s) : launch<128, false>(a, s);
-  return f16 ? launch<64, true>(a, s) : launch<64, false>(a, s);
+  const int max_keys = max_seqlen_k > 0 && max_seqlen_k < a.cap ? max_seqlen_k : a.cap;
+  if (head_dim == 128)
+    return f16 ? launch<128, true>(a, max_keys, s) : launch<128, false>(a, max_keys, s);
+  return f16 ? launch<64, true>(a, max_keys, s) : launch<64, false>(a, max_keys, s);
 }

@@ -9,7 +9,7 @@
 // lanes a row, and the rows of a workgroup are tokens of ONE head: their codes are neighbours
 // in the cache wherever their slots are.
 //
-// One row per thread: 16384 tokens x 8 heads x 128 of consecutive pages are stored in 19.7 us (4.5 TB/s;
+// One row per thread: 16384 tokens x 8 heads x 128 of consecutive pages are stored in 19.4 us (4.5 TB/s;
 // a copy of 1 GiB reaches 5.1) and read back, just written, in 14.5; 64 tokens in 3.1 and 2.9 us.
 // 2, 4 and 8 rows per thread: stored in 18.9 / 20.7 / 23.1 us, and 4096 tokens in 8.0 / 8.7 / 9.6
 // against 7.0.  The codes are read with plain loads: non-temporal ones take 5 % less time where the
@@ -187,7 +187,7 @@ __device__ void uniform_prefix(const Fp4Expand& a) {
 
 // Keys and values of each sequence's pages as f16 (see Fp4Expand).  grid = (pairs of heads, 16-token
 // pieces of a sequence, sequences); 16 lanes a row.  32 sequences of U{612..1536} tokens and 8 heads,
-// 31 MB read and 110 written: 39 us; with all heads of a piece in a workgroup 41, with one head 48, and
+// 37 MB read and 133 written: 36 us (pieces first 39); then, with all heads of a piece in a workgroup 41, with one head 48, and
 // other mappings (a quad per row, 4 heads of a token per wave, loads a step ahead) 41 to 48.
 template <bool F16>
 __global__ __launch_bounds__(256) void fp4_expand_kernel(Fp4Expand a) {

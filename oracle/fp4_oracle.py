@@ -73,9 +73,11 @@ def store(rows, data, scale, slots, keys):
             scale[slot // p, :, :, slot % p] = s[t]
 
 
-def through_pages(n, g, d):
-    """Whether n queries of g heads per kv head run over f16 pages of the keys and values."""
-    return n * g > 192 and d == 128 and g in (1, 2, 4, 8)
+def through_pages(n, g, d, groups, keys):
+    """Whether n queries of g heads per kv head run over f16 pages of the keys and values, in a call
+    of `groups` (sequence, kv head) pairs of at most `keys` keys."""
+    chunks = -(-n * g // 16) * -(-keys // 64) * groups
+    return n * g > 192 and d == 128 and g in (1, 2, 4, 8) and chunks >= 16384
 
 
 def attention(q, k, v, n_keys, scale, pages=False):

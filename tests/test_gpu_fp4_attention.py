@@ -13,11 +13,13 @@ from oracle import fp4_oracle as orc
 pytestmark = pytest.mark.gpu
 
 
-def _reference(q, pages, tables, n_queries, lens, scale, longest=None):
-    """Oracle of sequences whose queries follow each other in q [tokens, Hq, D]; longest: the most
-    queries that the call was told of."""
+def _reference(q, pages, tables, n_queries, lens, scale, keys=None):
+    """Oracle of sequences whose queries follow each other in q [tokens, Hq, D]; keys: the most that
+    the call was told of, what the table holds if none."""
     qn = q.double().cpu().numpy()
-    through = orc.through_pages(longest or max(n_queries), q.shape[1] // pages.hkv, pages.d)
+    keys = keys or len(tables[0]) * pages.bs
+    through = orc.through_pages(max(n_queries), q.shape[1] // pages.hkv, pages.d,
+                                len(lens) * pages.hkv, keys)
     out, size = np.zeros(qn.shape), np.zeros(qn.shape)
     at = 0
     for b, (n, m) in enumerate(zip(n_queries, lens)):
@@ -25,6 +27,13 @@ def _reference(q, pages, tables, n_queries, lens, scale, longest=None):
         out[at:at + n], size[at:at + n] = orc.attention(qn[at:at + n], k, v, m, scale, through)
         at += n
     return out, size
+
+
+def _wide(tables, bs, tokens):
+    """The tables with room for `tokens`: chunks enough for the route over f16 pages."""
+    wide = np.full((len(tables), -(-tokens // bs)), -1, np.int32)
+    wide[:, :tables.shape[1]] = tables
+    return wide
 
 
 def _int(a):
@@ -71,11 +80,13 @@ def test_several_queries_of_every_sequence(n, hq, hkv, d, dtype):
     pages = Pages(7, nb, 64, hkv, d, dtype)
     q = rng_rows(11, (len(lens), n, hq, d), dtype).cuda()
     say(f"fp4 {n} queries {hq}/{hkv} x {d} {dtype}")
-    out = flash_attn_with_kvcache(q, *pages.gpu(), cache_seqlens=_int(lens),
-                                  block_table=_int(tables), causal=True)
     ref, size = _reference(q.flatten(0, 1), pages, tables, [n] * len(lens), lens, d ** -0.5)
-    assert out.shape == q.shape
-    assert_close(out, ref, size, dtype, "fp4 several queries")
+    # a workgroup per group, and (tables that could hold more) ranges of chunks
+    for table in (tables, _wide(tables, 64, 5000)):
+        out = flash_attn_with_kvcache(q, *pages.gpu(), cache_seqlens=_int(lens),
+                                      block_table=_int(table), causal=True)
+        assert out.shape == q.shape
+        assert_close(out, ref, size, dtype, "fp4 several queries")
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
@@ -125,6 +136,32 @@ def test_tiles_of_32_rows(n, hq, hkv, d, bs, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("n,hq,hkv,d,bs,width", [(1, 16, 8, 128, 256, 0), (3, 16, 8, 128, 16, 0),
+                                                 (6, 16, 8, 128, 64, 0), (1, 16, 2, 128, 256, 0),
+                                                 (12, 16, 8, 128, 256, 65536), (2, 8, 8, 64, 32, 0),
+                                                 (20, 8, 8, 64, 64, 65536)])
+def test_several_chunks_for_every_wave(n, hq, hkv, d, bs, width, dtype):
+    """More chunks of 64 keys than the 2048 waves: groups that waves of a workgroup share, that
+    workgroups share, and whole ones.  (Caches of random codes; width: tokens that a table could hold.)"""
+    mean = 64 * 2900 // (6 * hkv)
+    lens = [int(mean * x) for x in (0.02, 1.9, 0.3, 1, 1.5, 0.7)] + [0, n]
+    tables, nb = tables_of(lens, bs, 4)
+    rng = np.random.default_rng(8)
+    pages = Pages.__new__(Pages)
+    pages.nb, pages.bs, pages.hkv, pages.d = nb, bs, hkv, d
+    pages.np = [(rng.integers(0, 256, (nb, hkv, bs, d // 2), dtype=np.uint8),
+                 rng.uniform(0.1, 0.4, (nb, hkv, d // 32, bs)).astype(np.float16)) for _ in range(2)]
+    wide = np.full((len(lens), max(width // bs, tables.shape[1])), -1, np.int32)
+    wide[:, :tables.shape[1]] = tables
+    q = rng_rows(11, (len(lens), n, hq, d), dtype).cuda()
+    say(f"fp4 {n} queries {hq}/{hkv} x {d} pages {bs} {dtype}, several chunks a wave")
+    out = flash_attn_with_kvcache(q, *pages.gpu(), cache_seqlens=_int(lens), block_table=_int(wide),
+                                  causal=True)
+    ref, size = _reference(q.flatten(0, 1), pages, tables, [n] * len(lens), lens, d ** -0.5)
+    assert_close(out, ref, size, dtype, "fp4 several chunks a wave")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
 @pytest.mark.parametrize("hq,hkv,d,bs", [(16, 8, 128, 256), (4, 1, 128, 16), (16, 16, 64, 48)])
 def test_one_workgroup_per_group_and_ranges_of_waves_agree(hq, hkv, d, bs, dtype):
     """Short contexts in one kernel; the same with a table that could hold more, cut between waves."""
@@ -148,14 +185,15 @@ def test_chunks_of_many_queries(hq, hkv, bs, dtype):
     news, cached = [200, 33, 0, 64, 40], [300, 0, 20, 65, -10]
     lens = [a + b for a, b in zip(news, cached)]
     tables, nb = tables_of(lens, bs, 8)
+    tables = _wide(tables, bs, 32768)
     pages = Pages(12, nb, bs, hkv, 128, dtype)
     q = rng_rows(13, (sum(news), hq, 128), dtype).cuda()
     cu = lambda v: _int(np.concatenate([[0], np.cumsum(v)]))
     say(f"fp4 chunks {hq}/{hkv} pages {bs} {dtype}")
-    for mk in (None, max(lens)):
+    for mk in (None, 20000, max(lens)):             # the last: without pages
         out = varlen_prefill(q, *pages.gpu(), cu(news), cu(lens), max(news), None,
                              block_table=_int(tables), max_seqlen_k=mk)
-        ref, size = _reference(q, pages, tables, news, lens, 128 ** -0.5)
+        ref, size = _reference(q, pages, tables, news, lens, 128 ** -0.5, mk)
         assert_close(out, ref, size, dtype, "fp4 chunks")
 
 
@@ -164,6 +202,7 @@ def test_chunks_of_queries_far_from_one(up):
     """bf16 queries outside f16's range, and values that only an eighth of fits it."""
     hq, hkv, n = 2, 1, 100
     tables, nb = tables_of([120], 64, 8)
+    tables = _wide(tables, 64, 98304)
     pages = Pages(12, nb, 64, hkv, 128)
     big = rng_rows(3, (nb * 64, hkv, 128), "bf16").double().numpy() * 2.0 ** 16
     orc.store(big, *pages.np[1], np.arange(nb * 64), False)
@@ -178,6 +217,7 @@ def test_chunks_of_queries_far_from_one(up):
 def test_chunks_do_not_see_what_is_not_finite_behind_the_mask():
     n, lens = 100, [130]
     tables, nb = tables_of(lens, 64, 4)
+    tables = _wide(tables, 64, 65536)
     pages = Pages(7, nb, 64, 2, 128)
     q = rng_rows(1, (n, 4, 128), "bf16").cuda()
     ref, size = _reference(q, pages, tables, [n], lens, 128 ** -0.5)
@@ -201,7 +241,7 @@ def test_a_batch_larger_than_the_pages_goes_in_parts():
     say("fp4 chunks in parts")
     out = flash_attn_with_kvcache(q, *pages.gpu(), cache_seqlens=_int(lens), block_table=_int(wide),
                                   causal=True)
-    ref, size = _reference(q.flatten(0, 1), pages, tables, [n] * len(lens), lens, 128 ** -0.5)
+    ref, size = _reference(q.flatten(0, 1), pages, wide, [n] * len(lens), lens, 128 ** -0.5)
     assert_close(out, ref, size, "bf16", "fp4 parts of a batch")
 
 
@@ -230,6 +270,7 @@ def test_a_chunk_over_more_keys_than_one_grid_dimension_holds():
 def test_a_captured_chunk_follows_its_inputs():
     lens, n = [130, 190], 100
     tables, nb = tables_of([190] * 2, 64, 3)
+    tables = _wide(tables, 64, 32768)
     pages = Pages(7, nb, 64, 2, 128)
     q, keys = rng_rows(1, (2, n, 4, 128), "bf16").cuda(), _int(lens)
     call = lambda: flash_attn_with_kvcache(q, *gpu, cache_seqlens=keys, block_table=bt, causal=True)

@@ -67,7 +67,7 @@ class _Model:
         """Oracle over what the caches hold."""
         qn, outs, sizes, at = q.double().cpu().numpy(), [], [], 0
         values = [orc.values(*self.np[i], keys=i == 0) for i in range(2)]
-        pages = orc.through_pages(max(news), HQ // HKV, HD)
+        pages = orc.through_pages(max(news), HQ // HKV, HD, len(news) * HKV, max(lens))
         for b, (n, m) in enumerate(zip(news, lens)):
             p = np.arange(m)
             rows = np.asarray(TABLES[b])[p // BS], p % BS
@@ -114,7 +114,7 @@ def test_a_layer_over_4_bit_caches():
         m.check_caches()
 
         # the next chunk of each, over what the caches hold; the module called by itself
-        for news in ([100, 1, 20], [3, 8, 1]):           # through f16 pages, and not
+        for news in ([100, 1, 20], [3, 8, 1]):
             lens = [a + b for a, b in zip(lens, news)]
             slots, pos = _prefill_context(news, lens, True)
             qkv = m.qkv(sum(news))
