@@ -24,7 +24,7 @@
 //     loaded once the scores have used these, its values and scales after P.V: there is always
 //     something in flight, and a second buffer for what goes to LDS gained nothing (64 x
 //     U{100..2048}, 16/8 heads: 23.1 us per call with two, 22.3 with one).
-// What bounds it.  64 x U{100..2048} keys, 16/8 heads (86 MB of codes and scales), 22 us: 4 us until the
+// What bounds it.  Ranges, 64 x U{100..2048} keys, 16/8 heads (86 MB of codes and scales), 22 us: 4 us until the
 // first chunk has come (prefix, position, page, data: four dependent round trips), 11 to 12 us of
 // stream at 5.7 to 6.4 TB/s, 4 us for the merging kernel and its launch.  Without the 128 conversions
 // of a chunk it is 1 % shorter, so it is not the arithmetic.  192 x U{256..4096}, 16/16 heads (922
@@ -65,6 +65,7 @@ struct AttnArgs {
   int32_t* desc;  // [batch][Hkv][max_tiles] x 2: first and last workgroup of the group, -1 if empty
   float* rec;     // [workgroups][2][rec_rows][HD + 4]: O, m, l
   int rec_rows, n_waves, wave_shift;  // n_waves = 2^wave_shift
+  int round;      // WHOLE: sequences whose groups fill the CUs once, 0: in their own order
 };
 
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
@@ -146,6 +147,51 @@ struct Split {
   }
 };
 
+// WHOLE, more groups than CUs: the sequence of place y, such that a CU's groups add up to much the same.
+// Places go to the CUs in rounds: by falling length in the first, third, ... round, by rising
+// length in those between.  (Every group's result is the same in any order.)  In their own order /
+// dealt out: 64 x U{100..2048}, 16/8 heads, 22.7 / 19.5 us, 100 x U{100..1500}, 16/4 heads, 17.9 / 14.9,
+// 64 x 6 queries over U{100..1024} 17.9 / 16.1; contexts of one length 29.6 / 30.5 (64 x 2048): it takes
+// 1 us, which up to 512 keys is not regained (64 x U{16..256} 7.2 / 8.4).
+constexpr int kBalanced = 128;  // sequences, two per lane
+template <int W>
+__device__ int balanced_place(const AttnArgs& a, int y, int lane, int wave, int (*s_count)[kBalanced]) {
+  const int round = y / a.round, p = y - round * a.round;
+  const int in_round = min(a.round, a.batch - round * a.round);
+  const int rank = round * a.round + (round & 1 ? in_round - 1 - p : p);
+  int key[2];  // chunks, then the lower number first: no two alike
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int s = lane + 64 * i;
+    key[i] = -1;
+    if (s < a.batch) {
+      const Seq x = seq_of(a, s);
+      key[i] = (x.queries > 0 ? chunks_of(x) : 0) * kBalanced + kBalanced - 1 - s;
+    }
+  }
+  int longer[2] = {0, 0};  // of this wave's share of the sequences
+  constexpr int kShare = kBalanced / W;
+#pragma unroll
+  for (int j = 0; j < kShare; ++j) {
+    const int c = wave * kShare + j;
+    const int k = __builtin_amdgcn_readlane(c < 64 ? key[0] : key[1], c & 63);
+    longer[0] += k > key[0];
+    longer[1] += k > key[1];
+  }
+  s_count[wave][lane] = longer[0];
+  s_count[wave][lane + 64] = longer[1];
+  __syncthreads();
+  int all[2] = {0, 0};
+#pragma unroll
+  for (int v = 0; v < W; ++v) {
+    all[0] += s_count[v][lane];
+    all[1] += s_count[v][lane + 64];
+  }
+  const uint64_t m = __builtin_amdgcn_ballot_w64(lane < a.batch && all[0] == rank);
+  if (m) return __builtin_ctzll(m);
+  return 64 + __builtin_ctzll(__builtin_amdgcn_ballot_w64(lane + 64 < a.batch && all[1] == rank));
+}
+
 // 16 bytes per lane straight into LDS: lane l writes [dst + 16 l, +16).  From base + the lane's
 // offset, or from the lane's own address.
 __device__ __forceinline__ void lds_load(const void* base, uint32_t offset, uint32_t dst) {
@@ -224,6 +270,7 @@ __global__ __launch_bounds__(64 * W, WHOLE ? (NC >= 4 || HD == 64 ? 4 : NC == 2 
   __shared__ nvk_f32x4 s_o[kFollow][WHOLE ? 1 : NT * 2 * NS][64];
   __shared__ float2 s_ml[kFollow][NT][64];
   __shared__ int s_ended[kFollow];
+  __shared__ int s_count[WHOLE ? W : 1][kBalanced];
   const int tid = threadIdx.x, lane = tid & 63;
   const int r = lane & 15, g = lane >> 4;
   const int Hkv = a.num_kv_heads;
@@ -236,6 +283,7 @@ __global__ __launch_bounds__(64 * W, WHOLE ? (NC >= 4 || HD == 64 ? 4 : NC == 2 
   if constexpr (WHOLE) {
     kvh = blockIdx.x;
     s = blockIdx.y;
+    if (a.round) s = uniform(balanced_place<W>(a, s, lane, wave, s_count));
     tile = blockIdx.z;
     sq = seq_of(a, s);
     n = uniform(chunks_of(sq));
@@ -913,8 +961,8 @@ bool plan_of(int batch, int max_queries, int num_q_heads, int num_kv_heads, int 
 //   20.5, 32 x 64 queries (2048) 47 / 42 / 66, 64 x 64 over U{600..1000} (4096) 88 / 93 / 149;
 //   up to 2048, ranges / 8 waves: 4 x 2048 (32) 9.7 / 12.4, but called one by one 15.7 / 12.7 (the second
 //   kernel is 3 us of the host's); 8 x 2048 (64) 11.8 / 12.5, 16 x U{100..2048} 14.6 / 13.1, 32 x 16.9 /
-//   14.3, 64 x 22.1 / 22.6, 64 x 2048 31.6 / 28.8, 128 x U{100..2048} (1024) 34.4 / 33.9; 6 queries: 32 x
-//   U{100..2048} 22.8 / 17.3, 64 x 29.3 / 31.0;
+//   14.3, 64 x 22.3 / 19.5, 64 x 2048 32.0 / 30.5, 128 x U{100..2048} (1024) 36.1 / 34.5; 6 queries: 32 x
+//   U{100..2048} 22.8 / 17.3, 48 x (384) 26.4 / 27.3;
 //   up to 4096: 32 x U{100..4096} 23.4 / 23.1, 32 x 4096 32.8 / 29.3, 16 x 4096 (128) 20.1 / 23.0, 48 x
 //   U{100..4096} (384) 28.6 / 35.7; up to 8192: 32 x U{100..8192} 35.5 / 40.9.
 constexpr int kCUs = 256;
@@ -942,15 +990,19 @@ int launch(const AttnArgs& a, int max_keys, hipStream_t s) {
   const int tiles16 = (rows + kR - 1) / kR;
   if (const int w =
           whole_waves(rows, HD, (int64_t)a.batch * a.num_kv_heads * tiles16, max_keys)) {
+    AttnArgs b = a;
+    const bool deal = (int64_t)a.batch * a.num_kv_heads > kCUs && tiles16 == 1 &&
+                      a.batch <= kBalanced && a.num_kv_heads <= kCUs && max_keys > 512;
+    b.round = deal ? kCUs / a.num_kv_heads : 0;
     const auto one_kernel = [&](auto nc, auto waves) {
       constexpr int NC = decltype(nc)::value, W = decltype(waves)::value;
       const dim3 groups(a.num_kv_heads, a.batch, tiles16);
       if (a.block_size % kCK)
         hipLaunchKernelGGL((fp4_attention_kernel<HD, F16, false, NC, 1, W, true>), groups,
-                           dim3(64 * W), 0, s, a);
+                           dim3(64 * W), 0, s, b);
       else
         hipLaunchKernelGGL((fp4_attention_kernel<HD, F16, true, NC, 1, W, true>), groups,
-                           dim3(64 * W), 0, s, a);
+                           dim3(64 * W), 0, s, b);
     };
     const auto by_rows = [&](auto waves) {
       if (rows <= kR / NG) one_kernel(few, waves);

@@ -187,8 +187,9 @@ __device__ void uniform_prefix(const Fp4Expand& a) {
 
 // Keys and values of each sequence's pages as f16 (see Fp4Expand).  grid = (pairs of heads, 16-token
 // pieces of a sequence, sequences); 16 lanes a row.  32 sequences of U{612..1536} tokens and 8 heads,
-// 37 MB read and 133 written: 36 us (pieces first 39); then, with all heads of a piece in a workgroup 41, with one head 48, and
-// other mappings (a quad per row, 4 heads of a token per wave, loads a step ahead) 41 to 48.
+// 37 MB read and 133 written: 33 to 36 us.  Pieces first 39; in that order all heads of a piece in a
+// workgroup 41, one head 48, and other mappings (a quad per row, 4 heads of a token per wave, loads a step
+// ahead) 41 to 48.
 template <bool F16>
 __global__ __launch_bounds__(256) void fp4_expand_kernel(Fp4Expand a) {
   constexpr int HD = 128, HB = 2;

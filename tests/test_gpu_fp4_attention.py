@@ -36,6 +36,16 @@ def _wide(tables, bs, tokens):
     return wide
 
 
+def _random_pages(seed, nb, bs, hkv, d):
+    """Caches of random codes and scales (nothing to quantise)."""
+    rng = np.random.default_rng(seed)
+    pages = Pages.__new__(Pages)
+    pages.nb, pages.bs, pages.hkv, pages.d = nb, bs, hkv, d
+    pages.np = [(rng.integers(0, 256, (nb, hkv, bs, d // 2), dtype=np.uint8),
+                 rng.uniform(0.1, 0.4, (nb, hkv, d // 32, bs)).astype(np.float16)) for _ in range(2)]
+    return pages
+
+
 def _int(a):
     return torch.as_tensor(np.asarray(a, dtype=np.int32)).cuda()
 
@@ -146,11 +156,7 @@ def test_several_chunks_for_every_wave(n, hq, hkv, d, bs, width, dtype):
     mean = 64 * 2900 // (6 * hkv)
     lens = [int(mean * x) for x in (0.02, 1.9, 0.3, 1, 1.5, 0.7)] + [0, n]
     tables, nb = tables_of(lens, bs, 4)
-    rng = np.random.default_rng(8)
-    pages = Pages.__new__(Pages)
-    pages.nb, pages.bs, pages.hkv, pages.d = nb, bs, hkv, d
-    pages.np = [(rng.integers(0, 256, (nb, hkv, bs, d // 2), dtype=np.uint8),
-                 rng.uniform(0.1, 0.4, (nb, hkv, d // 32, bs)).astype(np.float16)) for _ in range(2)]
+    pages = _random_pages(8, nb, bs, hkv, d)
     wide = np.full((len(lens), max(width // bs, tables.shape[1])), -1, np.int32)
     wide[:, :tables.shape[1]] = tables
     q = rng_rows(11, (len(lens), n, hq, d), dtype).cuda()
@@ -159,6 +165,31 @@ def test_several_chunks_for_every_wave(n, hq, hkv, d, bs, width, dtype):
                                   causal=True)
     ref, size = _reference(q.flatten(0, 1), pages, tables, [n] * len(lens), lens, d ** -0.5)
     assert_close(out, ref, size, dtype, "fp4 several chunks a wave")
+
+
+@pytest.mark.parametrize("batch,n,hq,hkv,d,most,ragged", [
+    (70, 1, 16, 8, 128, 1000, True), (40, 1, 16, 8, 128, 1500, True), (33, 3, 16, 8, 128, 700, True),
+    (64, 6, 16, 8, 128, 600, True), (128, 1, 3, 3, 128, 800, False), (128, 1, 6, 3, 64, 1300, True),
+    (129, 1, 4, 2, 128, 700, False), (2, 1, 256, 256, 64, 600, True), (3, 1, 130, 130, 64, 600, True)])
+def test_more_groups_than_cus_of_short_contexts(batch, n, hq, hkv, d, most, ragged):
+    """Sequences are dealt out by their length: every one of them once, whatever lengths are alike,
+    zero, or given with prefix sums that leave some without queries."""
+    rng = np.random.default_rng(batch)
+    lens = [int(x) for x in rng.integers(0, most // 64 // 3, batch) * 64 + rng.integers(0, 2, batch) * 3]
+    lens[1], lens[-1] = most, 0
+    news = [n if not ragged or i % 5 else 0 for i in range(batch)]
+    tables, nb = tables_of(lens, 64, 4)
+    pages = _random_pages(8, nb, 64, hkv, d)
+    q = rng_rows(11, (sum(news), hq, d), "bf16").cuda()
+    say(f"fp4 {batch} x {n} queries {hq}/{hkv} x {d}, dealt out by length")
+    if ragged:
+        cu = lambda v: _int(np.concatenate([[0], np.cumsum(v)]))
+        out = flash_attn_varlen_func(q, *pages.gpu(), cu(news), cu(lens), n, most, causal=True,
+                                     block_table=_int(tables))
+    else:
+        out = paged_decode(q, *pages.gpu(), _int(lens), _int(tables), None)
+    ref, size = _reference(q, pages, tables, news, lens, d ** -0.5)
+    assert_close(out, ref, size, "bf16", "fp4 dealt out by length")
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
