@@ -166,7 +166,7 @@ __device__ int balanced_place(const AttnArgs& a, int y, int lane, int wave, int 
     key[i] = -1;
     if (s < a.batch) {
       const Seq x = seq_of(a, s);
-      key[i] = (x.queries > 0 ? chunks_of(x) : 0) * kBalanced + kBalanced - 1 - s;
+      key[i] = (x.queries > 0 ? min(chunks_of(x), 1 << 20) : 0) * kBalanced + kBalanced - 1 - s;
     }
   }
   int longer[2] = {0, 0};  // of this wave's share of the sequences
